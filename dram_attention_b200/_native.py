@@ -81,6 +81,10 @@ _SIGNATURES = {
     "da_fork_destroy": (None, [c_void_p]),
     "da_build_pages": (c_int, [c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p,
                                c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "da_rotate": (c_int, [c_char_p]),
+    "da_append_pages": (c_int, [c_char_p]),
+    "da_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "da_paged_attention": (c_int, [c_char_p]),
 }
 
 _lib = None
@@ -114,6 +118,12 @@ def generate(*fields: int) -> None:
     code = lib().da_generate(_PACK(*fields, *(0,) * (_GENERATE_FIELDS - len(fields))))
     if code != 0:
         check(code, "da_generate")
+
+
+# argument blocks of the paged-cache calls: every field 8 bytes, in the header's order
+PACK_ROTATE = struct.Struct("=4q3q3q2q2q4qd7q").pack
+PACK_APPEND = struct.Struct("=4q6q5q3q2q2q3qd6q").pack
+PACK_ATTEND = struct.Struct("=3q5q3qq2qd4q6q").pack
 
 
 class Fork:

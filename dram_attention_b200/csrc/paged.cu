@@ -1,0 +1,215 @@
+// Attention over a paged cache: the join of the items that cross CTAs, and the host side.
+
+#include "paged_attn.cuh"
+
+namespace da {
+
+constexpr int kJoinWarps = 8;
+
+// One CTA per item and block of query rows.  `slices` warps share a row (each every slices-th partial result): all of them
+// when there are few rows and so, for a long line, many partial results of each; one per row when there are many rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int slices) {
+    constexpr int PW = PagedRow<D>::kWidth;
+    constexpr int NV = (D / 4 + 31) / 32;          // float4 columns per lane
+    constexpr int AHEAD = 4;
+    __shared__ float4 sh_o[kJoinWarps][D / 4];
+    __shared__ float2 sh_ml[kJoinWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int item = blockIdx.x;
+    const int per = p.n_kv_heads * p.groups, b = item / per;
+    const int row = blockIdx.y * (kJoinWarps / slices) + warp / slices, slice = warp % slices;
+    const int rows = rows_of(p, item);
+
+    // (the lengths were complete before the launch that this one follows let it in)
+    const Totals units = total_units(p, b, lane);
+    const int mine = span_of(p, __ldg(p.lengths + b)).units;
+    griddep_wait();
+    griddep_launch_dependents();
+    size_t index = 0;
+    T *out = out_row<T>(p, item, row < rows ? row : 0, D, index);
+    if (mine == 0) {                               // nothing to attend to
+        if (slice == 0 && row < rows) {
+            for (int c = lane; c < D; c += 32) out[c] = from_float<T>(0.f);
+            if (lane == 0 && p.lse) p.lse[index] = -INFINITY;
+        }
+        if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && __ldg(p.lengths + b) < 0) atomicOr(p.status, DA_STATUS_BAD_POSITION);
+        return;
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && __ldg(p.lengths + b) > p.capacity)
+        atomicOr(p.status, DA_STATUS_BAD_POSITION);
+    const long long begin = units.before + (long long)(item % per) * mine;
+    const int ctas = paged_ctas(p, units.all, kPagedCtas);
+    const int c0 = cta_of(units.all, ctas, begin), c1 = cta_of(units.all, ctas, begin + mine - 1);
+    if (c0 == c1) return;                          // one CTA had all of it
+
+    float m = -INFINITY, l = 0.f;
+    float4 o[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows) {
+        for (int first = c0 + slice; first <= c1; first += slices * AHEAD) {
+            float4 v[AHEAD][NV];
+            float2 w[AHEAD];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int c = min(first + a * slices, c1);
+                const float *src = p.cta_partials + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * p.group_rows + row) * PW;
+                w[a] = __ldcg(reinterpret_cast<const float2 *>(src + D));
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    v[a][i] = lane + 32 * i < D / 4 ? __ldcg(reinterpret_cast<const float4 *>(src) + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float mx = m;
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                if (first + a * slices > c1) w[a] = make_float2(-INFINITY, 0.f);
+                mx = fmaxf(mx, w[a].x);
+            }
+            const float ms = mx == -INFINITY ? 0.f : mx;
+            const float old = fast_exp2(m - ms);
+            m = mx;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) o[i].x *= old, o[i].y *= old, o[i].z *= old, o[i].w *= old;
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                if (w[a].x == -INFINITY) continue;
+                const float k = fast_exp2(w[a].x - ms);
+                l = fmaf(w[a].y, k, l);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    o[i].x = fmaf(v[a][i].x, k, o[i].x);
+                    o[i].y = fmaf(v[a][i].y, k, o[i].y);
+                    o[i].z = fmaf(v[a][i].z, k, o[i].z);
+                    o[i].w = fmaf(v[a][i].w, k, o[i].w);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (lane + 32 * i < D / 4) sh_o[warp][lane + 32 * i] = o[i];
+    if (lane == 0) sh_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (slice != 0 || row >= rows) return;
+    for (int s = 1; s < slices; ++s) m = fmaxf(m, sh_ml[warp + s].x);
+    const float ms = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < slices; ++s) {
+        const float2 w = sh_ml[warp + s];
+        const float k = fast_exp2(w.x - ms);
+        l = fmaf(w.y, k, l);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (lane + 32 * i >= D / 4) continue;
+            const float4 v = sh_o[warp + s][lane + 32 * i];
+            o[i].x = fmaf(v.x, k, o[i].x);
+            o[i].y = fmaf(v.y, k, o[i].y);
+            o[i].z = fmaf(v.z, k, o[i].z);
+            o[i].w = fmaf(v.w, k, o[i].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (lane + 32 * i >= D / 4) continue;
+        const float x[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) out[4 * (lane + 32 * i) + c] = from_float<T>(l > 0.f ? x[c] / l : 0.f);
+    }
+    if (lane == 0 && p.lse) p.lse[index] = natural_lse(m, l);
+}
+
+template <typename T, int D> static cudaError_t launch_join(const PagedParams &p, cudaStream_t stream) {
+    const long long items = (long long)p.n_sequences * p.n_kv_heads * p.groups;
+    const int slices = items * p.group_rows <= 8 * kPagedCtas ? kJoinWarps : 1;
+    const int per_cta = kJoinWarps / slices;
+    return launch_dependent(paged_join_kernel<T, D>, dim3((unsigned)items, (p.group_rows + per_cta - 1) / per_cta), dim3(kJoinWarps * 32),
+                            (size_t)0, stream, p, slices);
+}
+
+template <typename T> static cudaError_t join(const PagedParams &p, int head_dim, cudaStream_t stream) {
+    switch (head_dim) {
+    case 64: return launch_join<T, 64>(p, stream);
+    case 80: return launch_join<T, 80>(p, stream);
+    case 96: return launch_join<T, 96>(p, stream);
+    case 128: return launch_join<T, 128>(p, stream);
+    default: return launch_join<T, 256>(p, stream);
+    }
+}
+
+// Query rows of a KV head that share a pass over its keys and values: as equal groups as possible.
+static int group_rows(int64_t rep, int64_t head_dim, int64_t dtype) {
+    const int64_t most = dtype == DA_F32 ? paged_f32_rows((int)head_dim) : kPagedMmaRows;
+    const int64_t groups = (rep + most - 1) / most;
+    return (int)((rep + groups - 1) / groups);
+}
+
+static bool paged_head_dim(int64_t d) { return d == 64 || d == 80 || d == 96 || d == 128 || d == 256; }
+
+static bool paged_shape(int64_t rep, int64_t head_dim, int64_t dtype) {
+    return rep >= 1 && rep <= 256 && paged_head_dim(head_dim) && dtype >= DA_F32 && dtype <= DA_BF16;
+}
+
+}  // namespace da
+
+extern "C" size_t da_paged_attention_workspace_bytes(int rep, int head_dim, int dtype) {
+    using namespace da;
+    if (!paged_shape(rep, head_dim, dtype)) return 0;
+    return (size_t)kPagedCtas * (kPagedMaxWarps + 2) * group_rows(rep, head_dim, dtype) * (head_dim + 4) * sizeof(float);
+}
+
+extern "C" int da_paged_attention(const da_paged_attention_args *args) {
+    using namespace da;
+    if (!args) return DA_ERR_NULL;
+    const da_paged_attention_args &a = *args;
+    if (!a.q || !a.pages || !a.page_table || !a.lengths || !a.out || !a.workspace || !a.status) return DA_ERR_NULL;
+    if (a.dtype < DA_F32 || a.dtype > DA_BF16) return DA_ERR_DTYPE;
+    if (a.n_sequences < 1 || a.n_kv_heads < 1 || a.rep < 1 || a.page_size < 1 || a.n_pages < 1 || a.table_columns < 1 ||
+        a.window < 0 || a.n_sequences > 0x7fffffff || a.n_kv_heads > 1 << 16 || a.page_size > 1 << 20 || a.n_pages > 0x7fffffff ||
+        a.table_columns > 0x7fffffff || a.table_columns * a.page_size > 0x7fffff00 || a.window > 0x7fffffff)
+        return DA_ERR_SHAPE;
+    if (!paged_shape(a.rep, a.head_dim, a.dtype)) return DA_ERR_UNSUPPORTED;
+    const int esize = a.dtype == DA_F32 ? 4 : 2;
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.pages) | reinterpret_cast<uintptr_t>(a.out) |
+                           reinterpret_cast<uintptr_t>(a.workspace);
+    const uintptr_t words = reinterpret_cast<uintptr_t>(a.page_table) | reinterpret_cast<uintptr_t>(a.lengths) |
+                            reinterpret_cast<uintptr_t>(a.lse) | reinterpret_cast<uintptr_t>(a.status);
+    if ((rows & 15) || (words & 3) ||
+        (a.q_strides[0] | a.q_strides[1] | a.page_stride | a.page_head_stride) % (16 / esize))
+        return DA_ERR_ALIGN;
+    if (a.workspace_bytes < (int64_t)da_paged_attention_workspace_bytes((int)a.rep, (int)a.head_dim, (int)a.dtype)) return DA_ERR_WORKSPACE;
+
+    PagedParams p = {};
+    p.q = static_cast<const unsigned char *>(a.q), p.q_seq = a.q_strides[0], p.q_head = a.q_strides[1];
+    p.pages = static_cast<const unsigned char *>(a.pages);
+    p.page_stride = a.page_stride, p.page_head_stride = a.page_head_stride;
+    p.n_pages = (int)a.n_pages, p.page_size = (int)a.page_size;
+    p.table = a.page_table, p.table_stride = a.table_stride;
+    p.capacity = (int)(a.table_columns * a.page_size);
+    p.lengths = a.lengths, p.n_sequences = (int)a.n_sequences, p.window = (int)a.window;
+    p.out = static_cast<unsigned char *>(a.out), p.lse = a.lse, p.status = a.status;
+    p.n_kv_heads = (int)a.n_kv_heads, p.rep = (int)a.rep;
+    p.group_rows = group_rows(a.rep, a.head_dim, a.dtype);
+    p.groups = (p.rep + p.group_rows - 1) / p.group_rows;
+    if (a.n_sequences * a.n_kv_heads * p.groups > 0x7fffffff) return DA_ERR_SHAPE;
+    p.cta_partials = static_cast<float *>(a.workspace);
+    p.warp_partials = p.cta_partials + (size_t)kPagedCtas * 2 * p.group_rows * (a.head_dim + 4);
+    p.min_units = kPagedMaxWarps;
+    p.scale_log2 = (float)(a.scale * 1.4426950408889634);
+    cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
+    cudaError_t e;
+    switch (a.dtype) {
+    case DA_F32: e = paged_attention_f32(p, (int)a.head_dim, stream); break;
+    case DA_F16: e = paged_attention_f16(p, (int)a.head_dim, stream); break;
+    default: e = paged_attention_bf16(p, (int)a.head_dim, stream); break;
+    }
+    if (e != cudaSuccess) return (int)e;
+    switch (a.dtype) {
+    case DA_F32: return (int)join<float>(p, (int)a.head_dim, stream);
+    case DA_F16: return (int)join<__half>(p, (int)a.head_dim, stream);
+    default: return (int)join<__nv_bfloat16>(p, (int)a.head_dim, stream);
+    }
+}

@@ -1,0 +1,181 @@
+// Attention over a paged cache, 16-bit element types: the two products of a 16-token unit on tensor cores.
+//
+// A KV head has a handful of query rows, far below the 64 rows of the smallest tcgen05.mma tile, and memory is what bounds
+// the kernel; warp-level mma.sync m16n8k16 needs an eighth of the instructions of CUDA-core arithmetic and no more.
+//   S = Q K^T   A = query rows in registers, B = key rows by ldmatrix
+//   O += P V    A = the weights, straight from S's accumulators, B = value rows by ldmatrix.trans
+// A token's rows lie 16 bytes apart from a multiple of 128 bytes in shared memory, so that the eight row addresses of an
+// ldmatrix tile fall into distinct banks for every head size that is a multiple of 16.
+#pragma once
+
+#include "mma_sync.cuh"
+#include "paged_attn.cuh"
+
+namespace da {
+
+// FULL: up to 16 query rows; otherwise up to 8 (rows 8..15 of the tile are zero and nothing is kept of them).
+template <typename T, int D_, bool FULL>
+struct PagedMma {
+    using Elem = T;
+    static constexpr int kD = D_, kRows = FULL ? 16 : 8;
+    static constexpr int ROWB = kD * 2, kPitch = 2 * ROWB + 16;
+    static constexpr int KSTEPS = kD / 16, NT = kD / 8, NR = FULL ? 2 : 1;
+    static_assert(kD % 16 == 0, "whole k-steps");
+
+    struct State {
+        uint32_t q[NR][2][KSTEPS];    // A fragments: [row half][k half][k-step]
+        float m[NR], l[NR];           // row maximum (the same in the four lanes of a row), this lane's share of the weight sum
+        float o[NT][4];
+    };
+
+    __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int item, int rows, int lane) {
+        const int head0 = (item / p.groups) * p.rep + (item % p.groups) * p.group_rows;
+#pragma unroll
+        for (int half = 0; half < NR; ++half) {
+            const int r = (lane >> 2) + 8 * half;
+            const T *row = reinterpret_cast<const T *>(p.q) + b * p.q_seq + (head0 + (r < rows ? r : 0)) * p.q_head;
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) {
+                const uint32_t w0 = *reinterpret_cast<const uint32_t *>(row + 16 * ks + 2 * (lane & 3));
+                const uint32_t w1 = *reinterpret_cast<const uint32_t *>(row + 16 * ks + 8 + 2 * (lane & 3));
+                st.q[half][0][ks] = r < rows ? w0 : 0u;
+                st.q[half][1][ks] = r < rows ? w1 : 0u;
+            }
+            st.m[half] = -INFINITY;
+            st.l[half] = 0.f;
+        }
+#pragma unroll
+        for (int d = 0; d < NT; ++d) st.o[d][0] = st.o[d][1] = st.o[d][2] = st.o[d][3] = 0.f;
+    }
+
+    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[NR][2], uint32_t b0, uint32_t b1) {
+        if constexpr (FULL) MmaTraits<T>::mma16(d, a[0][0], a[1][0], a[0][1], a[1][1], b0, b1);
+        else MmaTraits<T>::mma(d, a[0][0], a[0][1], b0, b1);
+    }
+
+    __device__ __forceinline__ static void consume(State &st, const unsigned char *unit, uint32_t mask, int lane, float scale_log2) {
+        const int qd = lane & 3, tile = lane >> 3, tr = lane & 7;
+        // key tiles of a k-step: tokens 0..7 and 8..15, channels 0..7 and 8..15 of it
+        const unsigned char *keys = unit + ((tile >> 1) * 8 + tr) * kPitch + (tile & 1) * 16;
+        // value tiles of 16 channels, transposed by the load
+        const unsigned char *values = unit + ROWB + ((tile & 1) * 8 + tr) * kPitch + (tile >> 1) * 16;
+
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};   // odd k-steps: four chains instead of two
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+            uint32_t b[4], a[NR][2];
+            ldmatrix_x4(b, keys + ks * 32);
+#pragma unroll
+            for (int half = 0; half < NR; ++half) a[half][0] = st.q[half][0][ks], a[half][1] = st.q[half][1][ks];
+            mma(ks & 1 ? t0 : s0, a, b[0], b[1]);
+            mma(ks & 1 ? t1 : s1, a, b[2], b[3]);
+        }
+        uint32_t pa[NR][2];
+#pragma unroll
+        for (int half = 0; half < NR; ++half) {
+            // this lane: row lane / 4 + 8 * half, tokens 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
+            float v[4];
+            v[0] = s0[2 * half] + t0[2 * half], v[1] = s0[2 * half + 1] + t0[2 * half + 1];
+            v[2] = s1[2 * half] + t1[2 * half], v[3] = s1[2 * half + 1] + t1[2 * half + 1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool there = (mask >> (2 * qd + (i & 1) + 8 * (i >> 1))) & 1;
+                v[i] = there ? v[i] * scale_log2 : -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            mx = fmaxf(mx, __shfl_xor_sync(DA_FULL_MASK, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(DA_FULL_MASK, mx, 2));
+            const float m = fmaxf(st.m[half], mx);
+            const float ms = m == -INFINITY ? 0.f : m;
+            const float alpha = fast_exp2(st.m[half] - ms);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = fast_exp2(v[i] - ms);
+            st.l[half] = st.l[half] * alpha + ((v[0] + v[1]) + (v[2] + v[3]));
+            st.m[half] = m;
+            if (__any_sync(DA_FULL_MASK, alpha != 1.f)) {   // once the maxima have settled there is nothing to rescale
+#pragma unroll
+                for (int d = 0; d < NT; ++d) {
+                    st.o[d][2 * half] *= alpha;
+                    st.o[d][2 * half + 1] *= alpha;
+                }
+            }
+            pa[half][0] = MmaTraits<T>::pack(v[0], v[1]);
+            pa[half][1] = MmaTraits<T>::pack(v[2], v[3]);
+        }
+#pragma unroll
+        for (int d = 0; d < NT / 2; ++d) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, values + d * 32);
+            mma(st.o[2 * d], pa, b[0], b[1]);
+            mma(st.o[2 * d + 1], pa, b[2], b[3]);
+        }
+    }
+
+    __device__ __forceinline__ static float row_sum(float l) {
+        l += __shfl_xor_sync(DA_FULL_MASK, l, 1);
+        return l + __shfl_xor_sync(DA_FULL_MASK, l, 2);
+    }
+
+    __device__ __forceinline__ static void publish(State &st, float *dst, int lane, int rows) {
+        constexpr int PW = PagedRow<kD>::kWidth;
+        const int qd = lane & 3;
+#pragma unroll
+        for (int half = 0; half < NR; ++half) {
+            const float l = row_sum(st.l[half]);
+            const int r = (lane >> 2) + 8 * half;
+            if (r >= rows) continue;
+#pragma unroll
+            for (int d = 0; d < NT; ++d)
+                *reinterpret_cast<float2 *>(dst + r * PW + 8 * d + 2 * qd) = make_float2(st.o[d][2 * half], st.o[d][2 * half + 1]);
+            if (qd == 0) *reinterpret_cast<float2 *>(dst + r * PW + kD) = make_float2(st.m[half], l);
+        }
+    }
+
+    __device__ __forceinline__ static void write(State &st, const PagedParams &p, int item, int rows, int lane) {
+        const int qd = lane & 3;
+#pragma unroll
+        for (int half = 0; half < NR; ++half) {
+            const float l = row_sum(st.l[half]);
+            const int r = (lane >> 2) + 8 * half;
+            if (r >= rows) continue;
+            size_t index;
+            T *out = out_row<T>(p, item, r, kD, index);
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int d = 0; d < NT; ++d)
+                *reinterpret_cast<uint32_t *>(out + 8 * d + 2 * qd) =
+                    MmaTraits<T>::pack(st.o[d][2 * half] * inv, st.o[d][2 * half + 1] * inv);
+            if (qd == 0 && p.lse) p.lse[index] = natural_lse(st.m[half], l);
+        }
+    }
+};
+
+// Ring: as many stages of 16 tokens as fit, for 12 warps; the accumulators of 256 channels leave registers for 6.
+template <int D> struct PagedMmaShape {
+    static constexpr int kStage = kPagedUnit * (4 * D + 16);
+    static constexpr int kWarps = D > 128 ? 6 : 12;
+    static constexpr int kFit = (220 * 1024) / (kWarps * kStage);
+    static constexpr int kStages = kFit > 4 ? 4 : kFit;
+    static_assert(kStages >= 2, "");
+};
+
+template <typename T, int D, bool FULL>
+static cudaError_t launch_paged_mma(const PagedParams &p, cudaStream_t stream) {
+    using Shape = PagedMmaShape<D>;
+    return launch_paged<PagedMma<T, D, FULL>, Shape::kWarps, Shape::kStages>(p, stream);
+}
+
+template <typename T>
+static cudaError_t paged_mma(const PagedParams &p, int head_dim, cudaStream_t stream) {
+    const bool full = p.group_rows > 8;
+    switch (head_dim) {
+    case 64: return full ? launch_paged_mma<T, 64, true>(p, stream) : launch_paged_mma<T, 64, false>(p, stream);
+    case 80: return full ? launch_paged_mma<T, 80, true>(p, stream) : launch_paged_mma<T, 80, false>(p, stream);
+    case 96: return full ? launch_paged_mma<T, 96, true>(p, stream) : launch_paged_mma<T, 96, false>(p, stream);
+    case 128: return full ? launch_paged_mma<T, 128, true>(p, stream) : launch_paged_mma<T, 128, false>(p, stream);
+    default: return full ? launch_paged_mma<T, 256, true>(p, stream) : launch_paged_mma<T, 256, false>(p, stream);
+    }
+}
+
+}  // namespace da

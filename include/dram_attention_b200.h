@@ -623,6 +623,111 @@ DA_API int da_generate(const da_generate_args *args);
 DA_API int da_fork_create(void **fork);
 DA_API void da_fork_destroy(void *fork);
 
+/*
+ * Several sequences in one pool of pages (no counterpart in the reference, whose operator holds one sequence).
+ *
+ * A pool is n_kv_heads x n_pages pages of page_size tokens; inside a page every token is its key row, then its value row,
+ * head_dim elements each (the payload layout of dram_attention/lru_cache.py:121-142, so a slot table is such a pool).  Page j
+ * of head h begins at pages + h * page_head_stride + j * page_stride (elements).  Token t of sequence b lies in page
+ * page_table[b * table_stride + t / page_size], row t % page_size; the same page for every head.
+ *
+ * Argument blocks: every field is 8 bytes (pointer, int64 or double).  Strides are in elements; channels are contiguous.
+ */
+
+/*
+ * Rotary positions: per channel pair i < rotary_dim / 2 of every head a rotation by positions * inv_freq[i] times `factor`;
+ * the other channels are copied.  The pair is channels (2i, 2i + 1) when `interleaved`, else (i, i + rotary_dim / 2).
+ * `transposed` turns the sign of the angle: the gradient of q and k from that of q_out and k_out.  Angles are formed and reduced in
+ * 64 bits.  Either of q and k may be null.
+ *
+ * q, k         (n_batch, n_tokens, heads, head_dim), strides (batch, token, head)
+ * q_out, k_out (n_batch, n_tokens, heads, head_dim) contiguous; must not overlap the inputs
+ * positions    int32, or int64 when positions_64; strides (batch, token); any sign, magnitude below 2^31
+ * inv_freq     (rotary_dim / 2) float32
+ * Any alignment of whole elements; rows of 16-byte pieces are the fast path.  head_dim <= 512.
+ */
+typedef struct da_rotate_args {
+    const void *q, *k;
+    void *q_out, *k_out;
+    int64_t q_strides[3], k_strides[3];
+    const void *positions;
+    int64_t positions_64, position_strides[2];
+    const float *inv_freq;
+    int64_t rotary_dim, interleaved, transposed;
+    double factor;
+    int64_t n_batch, n_tokens, n_q_heads, n_kv_heads, head_dim, dtype;
+    da_stream_t stream;
+} da_rotate_args;
+DA_API int da_rotate(const da_rotate_args *args);
+
+/*
+ * Appends the keys and values of new tokens to a pool, the keys rotated on the way, and rotates the queries beside them.
+ *
+ * k, v         (n_rows, n_kv_heads, head_dim), strides (row, head)
+ * q, q_out     optional (n_rows, n_q_heads, head_dim); q_out contiguous, must not overlap the inputs; needs inv_freq
+ * starts       (n_sequences + 1) int32: rows [starts[b], starts[b + 1]) are sequence b's, in order; NULL: one row per sequence
+ * lengths      (n_sequences) int32: tokens each sequence holds AFTER the call; the new ones are its last.  0: not in use, its
+ *              rows are skipped
+ * inv_freq     (rotary_dim / 2) float32, or NULL: nothing is rotated.  The position is the token's place in its sequence
+ * Rows of no sequence write nothing to the pool; their rows of q_out are zero.  A position outside the table sets
+ * DA_STATUS_BAD_POSITION (the row counts as one of no sequence), a page outside the pool DA_STATUS_BAD_PAGE_ID (only q_out is
+ * written).  Two sequences must not append to the same page.
+ */
+typedef struct da_append_pages_args {
+    const void *q, *k, *v;
+    void *q_out;
+    int64_t q_strides[2], k_strides[2], v_strides[2];
+    void *pages;
+    int64_t page_stride, page_head_stride, page_size, n_pages;
+    const int32_t *page_table;
+    int64_t table_stride, table_columns;
+    const int32_t *lengths, *starts;
+    int64_t n_sequences, n_rows;
+    const float *inv_freq;
+    int64_t rotary_dim, interleaved;
+    double factor;
+    int64_t n_q_heads, n_kv_heads, head_dim, dtype;
+    int32_t *status;
+    da_stream_t stream;
+} da_append_pages_args;
+DA_API int da_append_pages(const da_append_pages_args *args);
+
+/*
+ * Attention of one new token per sequence over its pages:
+ *   out[b, hq] = softmax over t in [max(0, lengths[b] - window), lengths[b]) of scale * q[b, hq] . k_t, applied to v
+ * (window 0: from the first token on).  float32 softmax and accumulation; split over the tokens and joined in a fixed
+ * order.  lengths is read on the device: a captured call follows it.
+ *
+ * q            (n_sequences, n_kv_heads * rep, head_dim), strides (sequence, head)
+ * out          (n_sequences, n_kv_heads * rep, head_dim) contiguous; a sequence of length 0: zeros
+ * lse          optional (n_sequences, n_kv_heads * rep) float32: log-sum-exp of the scaled scores, -inf for length 0
+ * workspace    da_paged_attention_workspace_bytes() bytes, 16-byte aligned; holds nothing between calls, must not be shared by
+ *              calls that may run at the same time
+ * A page outside the pool sets DA_STATUS_BAD_PAGE_ID and its tokens are left out; a length outside [0, table_columns *
+ * page_size] sets DA_STATUS_BAD_POSITION and is cut to it.  Table entries of tokens that are not attended to are not read.
+ * Requires head_dim in {64, 80, 96, 128, 256}, rep <= 256; q, pages, out and their strides multiples of 16 bytes.
+ */
+typedef struct da_paged_attention_args {
+    const void *q;
+    int64_t q_strides[2];
+    const void *pages;
+    int64_t page_stride, page_head_stride, page_size, n_pages;
+    const int32_t *page_table;
+    int64_t table_stride, table_columns;
+    const int32_t *lengths;
+    int64_t n_sequences, window;
+    double scale;
+    void *out;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t *status;
+    int64_t n_kv_heads, rep, head_dim, dtype;
+    da_stream_t stream;
+} da_paged_attention_args;
+DA_API size_t da_paged_attention_workspace_bytes(int rep, int head_dim, int dtype);   /* 0: not a shape of the call */
+DA_API int da_paged_attention(const da_paged_attention_args *args);
+
 #ifdef __cplusplus
 }
 #endif
