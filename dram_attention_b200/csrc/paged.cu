@@ -4,28 +4,31 @@
 
 namespace da {
 
-constexpr int kJoinWarps = 8;
-
-// One CTA per item and block of query rows.  `slices` warps share a row (each every slices-th partial result): all of them
-// when there are few rows and so, for a long line, many partial results of each; one per row when there are many rows.
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p, int slices) {
-    constexpr int PW = PagedRow<D>::kWidth;
-    constexpr int NV = (D / 4 + 31) / 32;          // float4 columns per lane
-    constexpr int AHEAD = 4;
-    __shared__ float4 sh_o[kJoinWarps][D / 4];
-    __shared__ float2 sh_ml[kJoinWarps];
+// One CTA per item and block of query rows.  WARPS / rows per CTA warps share a row (each every so-many-th partial result):
+// 32 of them when there are few rows and so, for a long line, many partial results of each (148 results of a row are one
+// round trip to memory then); one per row when there are many.
+template <typename T, int D, int WARPS, int SLICES>
+__global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParams p) {
+    constexpr int PW = PagedRow<D>::kWidth, COLS = D / 4;
+    constexpr int NV = (COLS + 31) / 32;           // float4 columns per lane
+    constexpr int ROWS = WARPS / SLICES, AHEAD = 5;
+    __shared__ __align__(16) float sh_o[SLICES > 1 ? WARPS : 1][D];
+    __shared__ float2 sh_ml[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int item = blockIdx.x;
     const int per = p.n_kv_heads * p.groups, b = item / per;
-    const int row = blockIdx.y * (kJoinWarps / slices) + warp / slices, slice = warp % slices;
+    const int row = blockIdx.y * ROWS + warp / SLICES, slice = warp % SLICES;
     const int rows = rows_of(p, item);
 
     // (the lengths were complete before the launch that this one follows let it in)
     const Totals units = total_units(p, b, lane);
-    const int mine = span_of(p, __ldg(p.lengths + b)).units;
+    const int length = __ldg(p.lengths + b);
+    const int mine = span_of(p, length).units;
+    const long long begin = units.before + (long long)(item % per) * mine;
+    const int ctas = paged_ctas(p, units.all, kPagedCtas);
     griddep_wait();
     griddep_launch_dependents();
+    if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && (length < 0 || length > p.capacity)) atomicOr(p.status, DA_STATUS_BAD_POSITION);
     size_t index = 0;
     T *out = out_row<T>(p, item, row < rows ? row : 0, D, index);
     if (mine == 0) {                               // nothing to attend to
@@ -33,101 +36,69 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
             for (int c = lane; c < D; c += 32) out[c] = from_float<T>(0.f);
             if (lane == 0 && p.lse) p.lse[index] = -INFINITY;
         }
-        if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && __ldg(p.lengths + b) < 0) atomicOr(p.status, DA_STATUS_BAD_POSITION);
         return;
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && __ldg(p.lengths + b) > p.capacity)
-        atomicOr(p.status, DA_STATUS_BAD_POSITION);
-    const long long begin = units.before + (long long)(item % per) * mine;
-    const int ctas = paged_ctas(p, units.all, kPagedCtas);
     const int c0 = cta_of(units.all, ctas, begin), c1 = cta_of(units.all, ctas, begin + mine - 1);
     if (c0 == c1) return;                          // one CTA had all of it
 
-    float m = -INFINITY, l = 0.f;
-    float4 o[NV];
+    PartialSum x[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < NV; ++i) x[i].clear();
     if (row < rows) {
-        for (int first = c0 + slice; first <= c1; first += slices * AHEAD) {
-            float4 v[AHEAD][NV];
-            float2 w[AHEAD];
+        for (int first = c0 + slice; first <= c1; first += SLICES * AHEAD) {
+            float4 v[NV][AHEAD];
+            float2 ml[AHEAD];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
-                const int c = min(first + a * slices, c1);
+                const int c = min(first + a * SLICES, c1);
                 const float *src = p.cta_partials + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * p.group_rows + row) * PW;
-                w[a] = __ldcg(reinterpret_cast<const float2 *>(src + D));
+                ml[a] = __ldcg(reinterpret_cast<const float2 *>(src + D));
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    v[a][i] = lane + 32 * i < D / 4 ? __ldcg(reinterpret_cast<const float4 *>(src) + lane + 32 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[i][a] = __ldcg(reinterpret_cast<const float4 *>(src) + min(lane + 32 * i, COLS - 1));
+                if (first + a * SLICES > c1) ml[a] = make_float2(-INFINITY, 0.f);
             }
-            float mx = m;
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                if (first + a * slices > c1) w[a] = make_float2(-INFINITY, 0.f);
-                mx = fmaxf(mx, w[a].x);
-            }
-            const float ms = mx == -INFINITY ? 0.f : mx;
-            const float old = fast_exp2(m - ms);
-            m = mx;
-            l *= old;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) o[i].x *= old, o[i].y *= old, o[i].z *= old, o[i].w *= old;
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                if (w[a].x == -INFINITY) continue;
-                const float k = fast_exp2(w[a].x - ms);
-                l = fmaf(w[a].y, k, l);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    o[i].x = fmaf(v[a][i].x, k, o[i].x);
-                    o[i].y = fmaf(v[a][i].y, k, o[i].y);
-                    o[i].z = fmaf(v[a][i].z, k, o[i].z);
-                    o[i].w = fmaf(v[a][i].w, k, o[i].w);
-                }
-            }
+            for (int i = 0; i < NV; ++i) x[i].add(ml, v[i]);
         }
     }
+    if constexpr (SLICES == 1) {
+        if (row >= rows) return;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (lane + 32 * i < D / 4) sh_o[warp][lane + 32 * i] = o[i];
-    if (lane == 0) sh_ml[warp] = make_float2(m, l);
-    __syncthreads();
-    if (slice != 0 || row >= rows) return;
-    for (int s = 1; s < slices; ++s) m = fmaxf(m, sh_ml[warp + s].x);
-    const float ms = m == -INFINITY ? 0.f : m;
-    l = 0.f;
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < COLS) store_divided(out + 4 * (lane + 32 * i), x[i].o, x[i].l);
+        if (lane == 0 && p.lse) p.lse[index] = natural_lse(x[0].m, x[0].l);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < slices; ++s) {
-        const float2 w = sh_ml[warp + s];
-        const float k = fast_exp2(w.x - ms);
-        l = fmaf(w.y, k, l);
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < COLS) reinterpret_cast<float4 *>(sh_o[warp])[lane + 32 * i] = x[i].o;
+        if (lane == 0) sh_ml[warp] = make_float2(x[0].m, x[0].l);
+        __syncthreads();
+        // one row per CTA: a thread adds up one channel of all slices, a lane of each warp the weights of one
+        static_assert(ROWS == 1 && SLICES == 32, "");
+        const float2 w = sh_ml[lane];
+        float m = w.x;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (lane + 32 * i >= D / 4) continue;
-            const float4 v = sh_o[warp + s][lane + 32 * i];
-            o[i].x = fmaf(v.x, k, o[i].x);
-            o[i].y = fmaf(v.y, k, o[i].y);
-            o[i].z = fmaf(v.z, k, o[i].z);
-            o[i].w = fmaf(v.w, k, o[i].w);
-        }
+        for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(DA_FULL_MASK, m, off));
+        const float k = fast_exp2(w.x - (m == -INFINITY ? 0.f : m));
+        float l = w.y * k;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(DA_FULL_MASK, l, off);
+        const int c = threadIdx.x;
+        if (row >= rows || warp * 32 >= D) return;   // (whole warps: the weights travel by shuffles)
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < SLICES; ++i) sum = fmaf(sh_o[i][min(c, D - 1)], __shfl_sync(DA_FULL_MASK, k, i), sum);
+        if (c < D) out[c] = from_float<T>(l > 0.f ? sum / l : 0.f);
+        if (c == 0 && p.lse) p.lse[index] = natural_lse(m, l);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (lane + 32 * i >= D / 4) continue;
-        const float x[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) out[4 * (lane + 32 * i) + c] = from_float<T>(l > 0.f ? x[c] / l : 0.f);
-    }
-    if (lane == 0 && p.lse) p.lse[index] = natural_lse(m, l);
 }
 
 template <typename T, int D> static cudaError_t launch_join(const PagedParams &p, cudaStream_t stream) {
     const long long items = (long long)p.n_sequences * p.n_kv_heads * p.groups;
-    const int slices = items * p.group_rows <= 8 * kPagedCtas ? kJoinWarps : 1;
-    const int per_cta = kJoinWarps / slices;
-    return launch_dependent(paged_join_kernel<T, D>, dim3((unsigned)items, (p.group_rows + per_cta - 1) / per_cta), dim3(kJoinWarps * 32),
-                            (size_t)0, stream, p, slices);
+    if (items * p.group_rows <= 2 * kPagedCtas)
+        return launch_dependent(paged_join_kernel<T, D, 32, 32>, dim3((unsigned)items, p.group_rows), dim3(1024), (size_t)0, stream, p);
+    return launch_dependent(paged_join_kernel<T, D, 8, 1>, dim3((unsigned)items, (p.group_rows + 7) / 8), dim3(256), (size_t)0, stream, p);
 }
 
 template <typename T> static cudaError_t join(const PagedParams &p, int head_dim, cudaStream_t stream) {
@@ -189,6 +160,11 @@ extern "C" int da_paged_attention(const da_paged_attention_args *args) {
     p.n_pages = (int)a.n_pages, p.page_size = (int)a.page_size;
     p.table = a.page_table, p.table_stride = a.table_stride;
     p.capacity = (int)(a.table_columns * a.page_size);
+    // t / page_size for 0 <= t < 2^31 by a multiplication (Granlund and Montgomery): floor(2^(31 + l) / d) + 1 with 2^l >= d
+    int l = 0;
+    while ((1 << l) < p.page_size) ++l;
+    p.page_mul = (uint32_t)((1ull << (31 + l)) / (unsigned)p.page_size + 1);
+    p.page_shift = 31 + l;
     p.lengths = a.lengths, p.n_sequences = (int)a.n_sequences, p.window = (int)a.window;
     p.out = static_cast<unsigned char *>(a.out), p.lse = a.lse, p.status = a.status;
     p.n_kv_heads = (int)a.n_kv_heads, p.rep = (int)a.rep;

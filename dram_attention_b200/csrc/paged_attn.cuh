@@ -35,6 +35,8 @@ struct PagedParams {
     const int32_t *table;
     long long table_stride;
     int capacity;                     // tokens a row of the table has room for
+    uint32_t page_mul;                // t / page_size = (t * page_mul) >> page_shift
+    int page_shift;
     const int32_t *lengths;
     int n_sequences, window;
     unsigned char *out;
@@ -61,15 +63,28 @@ __device__ __forceinline__ Span span_of(const PagedParams &p, int length) {
     return s;
 }
 
-__device__ __forceinline__ long long shfl_up_64(long long v, int by) {
-    const int lo = __shfl_up_sync(DA_FULL_MASK, (int)(v & 0xffffffff), by);
-    const int hi = __shfl_up_sync(DA_FULL_MASK, (int)(v >> 32), by);
-    return ((long long)hi << 32) | (unsigned)lo;
-}
 __device__ __forceinline__ long long shfl_64(long long v, int from) {
     const int lo = __shfl_sync(DA_FULL_MASK, (int)(v & 0xffffffff), from);
     const int hi = __shfl_sync(DA_FULL_MASK, (int)(v >> 32), from);
     return ((long long)hi << 32) | (unsigned)lo;
+}
+// (a 64-bit division takes some hundred instructions; nearly every line is shorter than 2^32 / 148 units)
+__device__ __forceinline__ long long divide(long long n, long long d) {
+    if (((n | d) >> 32) == 0) return (long long)((uint32_t)n / (uint32_t)d);
+    return n / d;
+}
+
+// Units per lane and per (head, group) of 32 sequences from b0 on, and their inclusive sums.
+__device__ __forceinline__ long long scan_units(const PagedParams &p, int b0, int lane, int &mine) {
+    mine = b0 + lane < p.n_sequences ? span_of(p, __ldg(p.lengths + b0 + lane)).units : 0;
+    long long sum = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int lo = __shfl_up_sync(DA_FULL_MASK, (int)(sum & 0xffffffff), off);
+        const int hi = __shfl_up_sync(DA_FULL_MASK, (int)(sum >> 32), off);
+        if (lane >= off) sum += ((long long)hi << 32) | (unsigned)lo;
+    }
+    return sum;
 }
 
 // Units of the whole launch, and of the sequences in front of `before` (all warps of a CTA compute the same).
@@ -92,69 +107,64 @@ __device__ __forceinline__ Totals total_units(const PagedParams &p, int before, 
     return {all * per, front * per};
 }
 
-// Sequence that unit `at` of the line lies in, and the line's position of its first unit.
-__device__ __forceinline__ void find_sequence(const PagedParams &p, long long at, int lane, int &b, long long &start) {
-    const int per = p.n_kv_heads * p.groups;
-    long long front = 0;
-    for (int b0 = 0; b0 < p.n_sequences; b0 += 32) {
-        const long long mine = b0 + lane < p.n_sequences ? (long long)span_of(p, __ldg(p.lengths + b0 + lane)).units * per : 0;
-        long long sum = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long v = shfl_up_64(sum, off);
-            if (lane >= off) sum += v;
-        }
-        const unsigned past = __ballot_sync(DA_FULL_MASK, front + sum > at);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            b = b0 + l;
-            start = front + shfl_64(sum - mine, l);
-            return;
-        }
-        front += shfl_64(sum, 31);
-    }
-    b = p.n_sequences - 1;   // (not reached: `at` is below the total)
-    start = front;
-}
-
 // How the line is dealt out.  CTA c has the units [c * total / ctas, (c + 1) * total / ctas).
 __device__ __forceinline__ int paged_ctas(const PagedParams &p, long long total, int most) {
-    const long long want = (total + p.min_units - 1) / p.min_units;
+    const long long want = divide(total + p.min_units - 1, p.min_units);
     return (int)(want < most ? want : most);
 }
-__device__ __forceinline__ long long cta_begin(long long total, int ctas, int c) { return total * c / ctas; }
+__device__ __forceinline__ long long cta_begin(long long total, int ctas, int c) { return divide(total * c, ctas); }
 __device__ __forceinline__ int cta_of(long long total, int ctas, long long unit) {
-    return (int)(((unit + 1) * ctas - 1) / total);
+    return (int)divide((unit + 1) * ctas - 1, total);
 }
 
 template <int D> struct PagedRow { static constexpr int kWidth = D + 4; };   // accumulator, maximum, weight sum, padding
 
 // A place in the line.
 struct Cursor {
-    int b, item;                      // item: (head, group) inside the sequence
-    int u;                            // unit inside the sequence
+    int b, head, group;               // the item
+    int u, end;                       // unit inside the sequence, and the first behind its last
     Span s;
-};
-__device__ __forceinline__ void cursor_next(const PagedParams &p, Cursor &c) {
-    if (++c.u < c.s.u0 + c.s.units) return;
-    if (++c.item < p.n_kv_heads * p.groups) {
-        c.u = c.s.u0;
-        return;
+    __device__ __forceinline__ int id(const PagedParams &p) const { return (b * p.n_kv_heads + head) * p.groups + group; }
+    __device__ __forceinline__ void enter(const PagedParams &p, int sequence) {
+        b = sequence;
+        s = span_of(p, __ldg(p.lengths + b));
+        end = s.u0 + s.units;
     }
-    c.item = 0;
-    while (c.b + 1 < p.n_sequences) {
-        ++c.b;
-        c.s = span_of(p, __ldg(p.lengths + c.b));
-        if (c.s.units) break;
+    // to the next unit of the line (there is one)
+    __device__ __forceinline__ void next(const PagedParams &p) {
+        if (++u < end) return;
+        if (++group == p.groups) {
+            group = 0;
+            if (++head == p.n_kv_heads) {
+                head = 0;
+                do enter(p, b + 1);
+                while (s.units == 0 && b + 1 < p.n_sequences);
+            }
+        }
+        u = s.u0;
     }
-    c.u = c.s.u0;
-}
-
-// What a warp leaves to its CTA: a partial result of an item, and whether the item begins and ends in the warp's stretch.
-struct WarpPart {
-    int item;                         // (sequence, head, group), -1: none
-    bool begins, ends;
-    const float *rows;
+    // to unit `at` of the line, which has `total`; `first`, `first_sum` = scan_units of the first 32 sequences
+    __device__ __forceinline__ void seek(const PagedParams &p, long long at, int lane, int first, long long first_sum) {
+        const int per = p.n_kv_heads * p.groups;
+        long long front = 0, sum = first_sum;
+        int mine = first;
+        for (int b0 = 0;; b0 += 32) {
+            const unsigned past = __ballot_sync(DA_FULL_MASK, (front + sum) * per > at);
+            if (past || b0 + 32 >= p.n_sequences) {
+                const int l = past ? __ffs(past) - 1 : 31;
+                enter(p, min(b0 + l, p.n_sequences - 1));
+                front += shfl_64(sum - mine, l);
+                break;
+            }
+            front += shfl_64(sum, 31);
+            sum = scan_units(p, b0 + 32, lane, mine);
+        }
+        const long long inside = at - front * per;
+        const int item = (int)divide(inside, max(s.units, 1));
+        head = item / p.groups;
+        group = item - head * p.groups;
+        u = s.u0 + (int)(inside - (long long)item * s.units);
+    }
 };
 
 template <typename T> __device__ __forceinline__ T *out_row(const PagedParams &p, int item, int row, int D, size_t &index) {
@@ -166,6 +176,43 @@ __device__ __forceinline__ int rows_of(const PagedParams &p, int item) {
     return min(p.group_rows, p.rep - (item % p.groups) * p.group_rows);
 }
 __device__ __forceinline__ float natural_lse(float m, float l) { return (m + log2f(l)) * 0.6931471805599453f; }
+
+// Running sum of partial results (max, weight sum, four accumulator columns), several at a time so that their loads and
+// exponentials do not wait for one another.
+struct PartialSum {
+    float m, l;
+    float4 o;
+    __device__ __forceinline__ void clear() { m = -INFINITY, l = 0.f, o = make_float4(0.f, 0.f, 0.f, 0.f); }
+    template <int N> __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&v)[N]) {
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) mx = fmaxf(mx, ml[i].x);
+        const float ms = mx == -INFINITY ? 0.f : mx;
+        const float old = fast_exp2(m - ms);
+        m = mx;
+        l *= old;
+        o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float w = fast_exp2(ml[i].x - ms);     // (0 for one without tokens: its sums are zero)
+            l = fmaf(ml[i].y, w, l);
+            o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
+        }
+    }
+};
+
+// Four consecutive elements, divided by the weight sum.
+template <typename T> __device__ __forceinline__ void store_divided(T *dst, const float4 &o, float l) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(dst) = l > 0.f ? make_float4(o.x / l, o.y / l, o.z / l, o.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+        union { T t[4]; uint2 w; } x;
+        x.t[0] = from_float<T>(o.x * inv), x.t[1] = from_float<T>(o.y * inv);
+        x.t[2] = from_float<T>(o.z * inv), x.t[3] = from_float<T>(o.w * inv);
+        *reinterpret_cast<uint2 *>(dst) = x.w;
+    }
+}
 
 // Math: the arithmetic of a unit.  kD, kPitch (bytes of a token in shared memory), State, begin (query rows),
 // consume (one unit), publish (a partial result), write (a complete one).
@@ -179,13 +226,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t bars[WARPS][STAGES];
     __shared__ uint32_t masks[WARPS][STAGES];      // tokens of the unit that are there
-    __shared__ WarpPart parts[WARPS][2];           // in the order of the line
+    // What the warps leave to the CTA, in the order of the line: warp w its item that ended inside its stretch, if it had begun
+    // before (2 w, in global memory: the ring is busy), and its last one (2 w + 1, in its ring).
+    __shared__ int part_item[2 * WARPS];           // -1: none
+    __shared__ int part_flags[2 * WARPS];          // 1: the item begins in the warp's stretch, 2: it ends there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
-        parts[warp][0].item = parts[warp][1].item = -1;
+        part_item[2 * warp] = part_item[2 * warp + 1] = -1;
     }
     mbar_fence_init();
     __syncwarp();
@@ -193,75 +243,82 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     griddep_launch_dependents();
 
     // ---- this warp's stretch ------------------------------------------------------------
-    const long long total = total_units(p, 0, lane).all;
+    int first;
+    const long long first_sum = scan_units(p, 0, lane, first);
+    const long long total = p.n_sequences <= 32 ? shfl_64(first_sum, 31) * (p.n_kv_heads * p.groups) : total_units(p, 0, lane).all;
     const int ctas = paged_ctas(p, total, gridDim.x);
     if ((int)blockIdx.x >= ctas) return;
-    const long long lo = cta_begin(total, ctas, blockIdx.x), hi = cta_begin(total, ctas, blockIdx.x + 1);
-    const long long begin = lo + (hi - lo) * warp / WARPS;
-    const int count = (int)(lo + (hi - lo) * (warp + 1) / WARPS - begin);
+    const long long lo = cta_begin(total, ctas, blockIdx.x);
+    const int mine = (int)(cta_begin(total, ctas, blockIdx.x + 1) - lo);
+    const int skip = (int)divide((long long)mine * warp, WARPS);
+    const int count = (int)divide((long long)mine * (warp + 1), WARPS) - skip;
     unsigned char *ring = smem + (size_t)warp * STAGES * STAGEB;
 
     if (count > 0) {
         Cursor ahead;
-        long long start;
-        find_sequence(p, begin, lane, ahead.b, start);
-        ahead.s = span_of(p, __ldg(p.lengths + ahead.b));
-        ahead.item = (int)((begin - start) / ahead.s.units);
-        ahead.u = ahead.s.u0 + (int)((begin - start) % ahead.s.units);
+        ahead.seek(p, lo + skip, lane, first, first_sum);
         Cursor at = ahead;
         bool begins = at.u == at.s.u0;
 
-        // a lane's token of the unit: the page it lies in, and its place there
+        // A lane's token of the unit to be requested next: its page (looked up one unit ahead), then its address.
         int page, slot;
         auto look_up = [&](const Cursor &c) {
             const int t = c.u * kPagedUnit + lane;
             page = -2;                             // no such token
             slot = 0;
             if (lane < kPagedUnit && t >= c.s.first && t < c.s.n) {
-                const int column = t / p.page_size;
+                const int column = (int)(((unsigned long long)(unsigned)t * p.page_mul) >> p.page_shift);
                 slot = t - column * p.page_size;
                 page = __ldg(p.table + c.b * p.table_stride + column);
                 if (page < 0 || page >= p.n_pages) page = -1;
             }
         };
-        auto issue = [&](const Cursor &c, int s) {
+        // Read once per call: the stream must not push the code of the joins and the partial results out of L2 (1.3 GB:
+        // 204 -> 200 us).
+        const uint64_t policy = l2_policy_evict_first();
+        const unsigned char *src;
+        uint32_t there;
+        auto locate = [&](const Cursor &c) {
             if (page == -1) atomicOr(p.status, DA_STATUS_BAD_PAGE_ID);   // the token is left out
-            const unsigned mask = __ballot_sync(DA_FULL_MASK, page >= 0);
+            there = __ballot_sync(DA_FULL_MASK, page >= 0);
+            src = p.pages + (c.head * p.page_head_stride + page * p.page_stride + slot * (2 * D)) * (long long)sizeof(T);
+        };
+        auto request = [&](int s) {
             if (lane == 0) {
-                masks[warp][s] = mask;
-                mbar_arrive_expect_tx(&bars[warp][s], (uint32_t)__popc(mask) * TOKB);
+                masks[warp][s] = there;
+                mbar_arrive_expect_tx(&bars[warp][s], (uint32_t)__popc(there) * TOKB);
             }
             __syncwarp();
-            if (page >= 0) {
-                const unsigned char *src = p.pages + ((c.item / p.groups) * p.page_head_stride + page * p.page_stride +
-                                                      (long long)slot * 2 * D) * (long long)sizeof(T);
-                bulk_copy_g2s(ring + s * STAGEB + lane * Math::kPitch, src, TOKB, &bars[warp][s]);
-            }
+            if (page >= 0) bulk_copy_g2s_hint(ring + s * STAGEB + lane * Math::kPitch, src, TOKB, &bars[warp][s], policy);
         };
 
         int issued = 0;
         look_up(ahead);
         for (; issued < STAGES && issued < count; ++issued) {
-            issue(ahead, issued);
+            locate(ahead);
+            request(issued);
             if (issued + 1 < count) {
-                cursor_next(p, ahead);
+                ahead.next(p);
                 look_up(ahead);
             }
         }
 
         typename Math::State st;
-        int id = at.b * (p.n_kv_heads * p.groups) + at.item;
+        int id = at.id(p);
         int rows = rows_of(p, id);
-        Math::begin(st, p, at.b, at.item, rows, lane);
-        int in_flight_from = 0;
-        bool dead = false;
+        Math::begin(st, p, at.b, at.head, at.group, rows, lane);
+        int s = 0;
+        uint32_t parity = 0;
         for (int i = 0; i < count; ++i) {
-            const int s = i % STAGES;
-            const bool arrived = mbar_wait_bounded(&bars[warp][s], (uint32_t)((i / STAGES) & 1));
+            if (issued < count) locate(ahead);
+            const bool arrived = mbar_wait_bounded(&bars[warp][s], parity);
             if (!__all_sync(DA_FULL_MASK, arrived)) {
                 if (lane == 0) atomicOr(p.status, DA_STATUS_WAIT_TIMEOUT);
-                dead = true;
-                in_flight_from = i;
+                // the copies under way end before the shared memory is given up, or the wait for them does
+                for (; i < issued; ++i) {
+                    mbar_wait_bounded(&bars[warp][s], parity);
+                    if (++s == STAGES) s = 0, parity ^= 1;
+                }
                 break;
             }
             unsigned char *unit = ring + s * STAGEB;
@@ -279,13 +336,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             Math::consume(st, unit, mask, lane, p.scale_log2);
             __syncwarp();
             if (issued < count) {
-                issue(ahead, issued % STAGES);
+                request(s);
                 if (++issued < count) {
-                    cursor_next(p, ahead);
+                    ahead.next(p);
                     look_up(ahead);
                 }
             }
-            const bool ends = at.u + 1 == at.s.u0 + at.s.units;
+            if (++s == STAGES) s = 0, parity ^= 1;
+            const bool ends = at.u + 1 == at.end;
             if (!ends && i + 1 < count) {
                 ++at.u;
                 continue;
@@ -294,73 +352,78 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             if (begins && ends) {
                 Math::write(st, p, id, rows, lane);
             } else {
-                const bool last = i + 1 == count;
-                float *dst = last ? reinterpret_cast<float *>(ring)
-                                  : p.warp_partials + ((size_t)blockIdx.x * WARPS + warp) * p.group_rows * PW;
+                const int k = 2 * warp + (i + 1 == count);
+                float *dst = i + 1 == count ? reinterpret_cast<float *>(ring)
+                                            : p.warp_partials + ((size_t)blockIdx.x * WARPS + warp) * p.group_rows * PW;
                 Math::publish(st, dst, lane, rows);
-                if (lane == 0) parts[warp][last ? 1 : 0] = {id, begins, ends, dst};
+                if (lane == 0) {
+                    part_item[k] = id;
+                    part_flags[k] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                }
             }
             if (i + 1 < count) {
-                cursor_next(p, at);
-                id = at.b * (p.n_kv_heads * p.groups) + at.item;
+                at.next(p);
+                id = at.id(p);
                 rows = rows_of(p, id);
                 begins = true;
-                Math::begin(st, p, at.b, at.item, rows, lane);
+                Math::begin(st, p, at.b, at.head, at.group, rows, lane);
             }
         }
-        if (dead)   // the copies under way end before the shared memory is given up, or the wait for them does
-            for (int i = in_flight_from; i < issued; ++i) mbar_wait_bounded(&bars[warp][i % STAGES], (uint32_t)((i / STAGES) & 1));
     }
     __syncthreads();
 
-    // ---- items that cross warps -------------------------------------------------------------
-    int k = 0;
-    while (k < 2 * WARPS) {
-        const WarpPart lead = parts[k >> 1][k & 1];
-        if (lead.item < 0) {
-            ++k;
-            continue;
-        }
-        int end = k + 1;
-        bool ends = lead.ends;
-        for (int j = k + 1; j < 2 * WARPS; ++j) {
-            const WarpPart &x = parts[j >> 1][j & 1];
-            if (x.item < 0) continue;
-            if (x.item != lead.item) break;
-            end = j + 1;
-            ends = x.ends;
-        }
-        const bool complete = lead.begins && ends;
-        const int rows = rows_of(p, lead.item);
-        float *dst = p.cta_partials + ((size_t)blockIdx.x * 2 + (lead.begins ? 1 : 0)) * p.group_rows * PW;
-        for (int e = tid; e < rows * PW; e += WARPS * 32) {
-            const int r = e / PW, c = e % PW;
-            float m = -INFINITY;
-            for (int j = k; j < end; ++j) {
-                const WarpPart &x = parts[j >> 1][j & 1];
-                if (x.item >= 0) m = fmaxf(m, x.rows[r * PW + D]);
+    // ---- items that cross warps: one task per item, row and four channels ------------------------------
+    constexpr int COLS = D / 4;
+    const int item_of = lane < 2 * WARPS ? part_item[lane] : -1;
+    const unsigned there = __ballot_sync(DA_FULL_MASK, item_of >= 0);
+    const unsigned in_front = there & ((1u << lane) - 1);
+    const int item_before = __shfl_sync(DA_FULL_MASK, item_of, in_front ? 31 - __clz(in_front) : 0);
+    unsigned leads = __ballot_sync(DA_FULL_MASK, item_of >= 0 && (!in_front || item_before != item_of));
+    const int n_items = __popc(leads);
+    const int tasks = p.group_rows * COLS;
+    int at_item = 0;                               // leads: from this item on
+    for (int t = tid; t < n_items * tasks; t += WARPS * 32) {
+        const int g = t / tasks, e = t - g * tasks;
+        const int r = e / COLS, c = e - r * COLS;
+        for (; at_item < g; ++at_item) leads &= leads - 1;
+        const int begin = __ffs(leads) - 1;
+        const unsigned behind = leads & (leads - 1);
+        unsigned parts = there & ~((1u << begin) - 1);
+        if (behind) parts &= (behind & -behind) - 1;
+        const int id = part_item[begin];
+        if (r >= rows_of(p, id)) continue;
+        const bool begins = part_flags[begin] & 1, ends = part_flags[31 - __clz(parts)] & 2;
+        PartialSum x;
+        x.clear();
+        while (parts) {
+            constexpr int N = 4;
+            float2 ml[N];
+            float4 v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                ml[i] = make_float2(-INFINITY, 0.f);
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (parts) {
+                    const int k = __ffs(parts) - 1;
+                    parts &= parts - 1;
+                    const float *row = (k & 1 ? reinterpret_cast<const float *>(smem + (size_t)(k >> 1) * STAGES * STAGEB)
+                                              : p.warp_partials + ((size_t)blockIdx.x * WARPS + (k >> 1)) * p.group_rows * PW) + r * PW;
+                    ml[i] = *reinterpret_cast<const float2 *>(row + D);
+                    v[i] = *reinterpret_cast<const float4 *>(row + 4 * c);
+                }
             }
-            const float ms = m == -INFINITY ? 0.f : m;
-            float sum = 0.f, l = 0.f;
-            for (int j = k; j < end; ++j) {
-                const WarpPart &x = parts[j >> 1][j & 1];
-                if (x.item < 0) continue;
-                const float w = fast_exp2(x.rows[r * PW + D] - ms);
-                sum = fmaf(x.rows[r * PW + min(c, D + 1)], w, sum);
-                l = fmaf(x.rows[r * PW + D + 1], w, l);
-            }
-            if (!complete) {
-                dst[e] = c == D ? m : sum;
-            } else if (c < D) {
-                size_t index;
-                out_row<T>(p, lead.item, r, D, index)[c] = from_float<T>(l > 0.f ? sum / l : 0.f);
-            } else if (c == D && p.lse) {
-                size_t index;
-                out_row<T>(p, lead.item, r, D, index);
-                p.lse[index] = natural_lse(m, l);
-            }
+            x.add(ml, v);
         }
-        k = end;
+        if (begins && ends) {
+            size_t index;
+            T *out = out_row<T>(p, id, r, D, index);
+            store_divided(out + 4 * c, x.o, x.l);
+            if (c == 0 && p.lse) p.lse[index] = natural_lse(x.m, x.l);
+        } else {
+            float *dst = p.cta_partials + (((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * p.group_rows + r) * PW;
+            *reinterpret_cast<float4 *>(dst + 4 * c) = x.o;
+            if (c == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(x.m, x.l);
+        }
     }
 }
 
@@ -382,7 +445,7 @@ static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
     return launch_dependent(kernel, dim3(kPagedCtas), dim3(WARPS * 32), (size_t)SMEM, stream, p);
 }
 
-constexpr int kPagedMaxWarps = 12;
+constexpr int kPagedMaxWarps = 8;
 // query rows that share a pass over the keys and values, float32: what the registers of a warp hold
 constexpr int paged_f32_rows(int head_dim) { return head_dim <= 64 ? 8 : (head_dim <= 128 ? 4 : 2); }
 constexpr int kPagedMmaRows = 16;

@@ -21,9 +21,9 @@ struct PagedSimt {
 
     __device__ __forceinline__ static bool has(int j, int i) { return PIECES % 8 == 0 || j + 8 * i < PIECES; }
 
-    __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int item, int rows, int lane) {
+    __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int head, int group, int rows, int lane) {
         const int j = lane & 7;
-        const int head0 = (item / p.groups) * p.rep + (item % p.groups) * p.group_rows;
+        const int head0 = head * p.rep + group * p.group_rows;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float *row = reinterpret_cast<const float *>(p.q) + b * p.q_seq + (head0 + (r < rows ? r : 0)) * p.q_head;
@@ -166,13 +166,27 @@ struct PagedSimt {
     }
 };
 
+// As few rows as the group has: fewer instructions per unit, and less code, which a short call fetches from memory.
+// (warps x stages x 16 tokens of 8 D bytes: 160 to 197 KB; more than 8 warps would have 168 registers)
+template <int D, int WARPS, int STAGES> static cudaError_t paged_simt(const PagedParams &p, cudaStream_t stream) {
+    constexpr int MOST = paged_f32_rows(D);
+    if (p.group_rows <= 1) return launch_paged<PagedSimt<D, 1>, WARPS, STAGES>(p, stream);
+    if constexpr (MOST > 2) {
+        if (p.group_rows <= 2) return launch_paged<PagedSimt<D, 2>, WARPS, STAGES>(p, stream);
+    }
+    if constexpr (MOST > 4) {
+        if (p.group_rows <= 4) return launch_paged<PagedSimt<D, 4>, WARPS, STAGES>(p, stream);
+    }
+    return launch_paged<PagedSimt<D, MOST>, WARPS, STAGES>(p, stream);
+}
+
 cudaError_t paged_attention_f32(const PagedParams &p, int head_dim, cudaStream_t stream) {
-    switch (head_dim) {   // (warps x stages x 16 tokens of 8 D bytes: 160 to 197 KB; more than 8 warps would have 168 registers)
-    case 64: return launch_paged<PagedSimt<64, paged_f32_rows(64)>, 8, 3>(p, stream);
-    case 80: return launch_paged<PagedSimt<80, paged_f32_rows(80)>, 8, 2>(p, stream);
-    case 96: return launch_paged<PagedSimt<96, paged_f32_rows(96)>, 8, 2>(p, stream);
-    case 128: return launch_paged<PagedSimt<128, paged_f32_rows(128)>, 6, 2>(p, stream);
-    default: return launch_paged<PagedSimt<256, paged_f32_rows(256)>, 3, 2>(p, stream);
+    switch (head_dim) {
+    case 64: return paged_simt<64, 8, 3>(p, stream);
+    case 80: return paged_simt<80, 8, 2>(p, stream);
+    case 96: return paged_simt<96, 8, 2>(p, stream);
+    case 128: return paged_simt<128, 6, 2>(p, stream);
+    default: return paged_simt<256, 3, 2>(p, stream);
     }
 }
 
