@@ -126,6 +126,22 @@ PACK_APPEND = struct.Struct("=4q6q5q3q2q2q3qd6q").pack
 PACK_ATTEND = struct.Struct("=3q5q3qq2qd4q6q").pack
 
 
+def launch(function, block: bytes, device: int, what: str) -> None:
+    """A call of the library that takes one argument block, with `device` current."""
+    if torch._C._cuda_getDevice() == device:
+        code = function(block)
+    else:
+        with torch.cuda.device(device):
+            code = function(block)
+    if code != 0:
+        check(code, what)
+
+
+def stream_of(device: int) -> int:
+    """cudaStream_t of torch's current stream on a device."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 class Fork:
     """Side stream and events of the two-launch layout, on the device current at construction."""
 

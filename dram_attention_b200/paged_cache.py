@@ -60,35 +60,44 @@ class PagedKVCache:
         self.n_kv_heads, self.n_pages, self.page_size, _, self.head_dim = pages.shape
         # (the stride of a dimension of one entry is never followed)
         head, page = pages.stride()[:2]
-        self._strides = (page if self.n_pages > 1 else 0, head if self.n_kv_heads > 1 else 0)
+        self._pool = (self.pages.data_ptr(), page if self.n_pages > 1 else 0, head if self.n_kv_heads > 1 else 0, self.page_size,
+                      self.n_pages)
+        self._device, self._dtype, self._dtype_code, self._piece = pages.get_device(), pages.dtype, _native.dtype_code(pages.dtype), piece
+        self._scratch = {}
         self.status = torch.zeros(1, dtype=torch.int32, device=pages.device)
 
     # ---- checks shared by the calls --------------------------------------------------------
     def _check_heads(self, t: torch.Tensor, name: str, rows: Optional[int], heads: Optional[int]) -> torch.Tensor:
-        assert t.dim() == 3 and t.shape[2] == self.head_dim and (rows is None or t.shape[0] == rows) and \
-            (heads is None or t.shape[1] == heads), \
-            f"{name} must be ({'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {self.head_dim}), got {tuple(t.shape)}"
-        self._check_device(t, name)
-        assert t.dtype == self.pages.dtype, f"{name} must be {self.pages.dtype} like the pages, got {t.dtype}"
+        shape = t.shape
+        assert len(shape) == 3 and shape[2] == self.head_dim and (rows is None or shape[0] == rows) and \
+            (heads is None or shape[1] == heads), \
+            f"{name} must be ({'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {self.head_dim}), got {tuple(shape)}"
+        if t.get_device() != self._device:
+            self._wrong_device(t, name)
+        assert t.dtype is self._dtype, f"{name} must be {self._dtype} like the pages, got {t.dtype}"
         assert not (t.requires_grad and torch.is_grad_enabled()), \
             f"{name} requires a gradient, which the paged cache does not pass on: detach it or call under torch.no_grad()"
         return t if t.stride(2) == 1 else t.contiguous()
 
-    def _check_device(self, t: torch.Tensor, name: str) -> None:
+    def _wrong_device(self, t: torch.Tensor, name: str) -> None:
         _native.require_cuda(t, name)
-        assert t.device == self.pages.device, f"{name} must be on the device of the pages ({self.pages.device}), got {t.device}"
+        raise AssertionError(f"{name} must be on the device of the pages ({self.pages.device}), got {t.device}")
 
-    def _check_table(self, page_table: torch.Tensor, lengths: torch.Tensor) -> int:
-        assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[1] > 0, \
-            f"page_table must be (n_sequences, columns) int32, got {tuple(page_table.shape)} {page_table.dtype}"
-        n = page_table.shape[0]
-        assert lengths.dtype == torch.int32 and lengths.shape == (n,), \
+    def _check_table(self, page_table: torch.Tensor, lengths: torch.Tensor):
+        """Sequences, columns and row stride of the table"""
+        shape, strides = page_table.shape, page_table.stride()
+        assert len(shape) == 2 and shape[1] > 0 and page_table.dtype is torch.int32, \
+            f"page_table must be (n_sequences, columns) int32, got {tuple(shape)} {page_table.dtype}"
+        n, columns = shape
+        assert lengths.dtype is torch.int32 and lengths.shape == (n,), \
             f"lengths must be ({n},) int32, got {tuple(lengths.shape)} {lengths.dtype}"
-        assert (page_table.shape[1] == 1 or page_table.stride(1) == 1) and (n <= 1 or lengths.stride(0) == 1), \
+        assert (strides[1] == 1 or columns == 1) and (n <= 1 or lengths.stride(0) == 1), \
             "the rows of page_table and lengths must be contiguous"
-        self._check_device(page_table, "page_table")
-        self._check_device(lengths, "lengths")
-        return n
+        if page_table.get_device() != self._device:
+            self._wrong_device(page_table, "page_table")
+        if lengths.get_device() != self._device:
+            self._wrong_device(lengths, "lengths")
+        return n, columns, strides[0]
 
     # ---- operators ----------------------------------------------------------------------------
     def append_(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
@@ -103,39 +112,40 @@ class PagedKVCache:
         q (rows, Hq, D), only with `rotary`: returned rotated like the keys (a new tensor; rows left out are zero).
         Two sequences must not append to the same page.  A position outside the table or a page outside the pool writes
         nothing and is reported by `check_status`."""
-        n = self._check_table(page_table, lengths)
+        n, columns, table_stride = self._check_table(page_table, lengths)
         k = self._check_heads(k, "k", None, self.n_kv_heads)
-        v = self._check_heads(v, "v", k.shape[0], self.n_kv_heads)
         rows = k.shape[0]
+        v = self._check_heads(v, "v", rows, self.n_kv_heads)
         if starts is None:
             assert rows == n, f"one row per sequence expected ({n}), got {rows}; pass starts for a ragged batch"
+            starts_ptr = 0
         else:
-            assert starts.dtype == torch.int32 and starts.shape == (n + 1,) and (n == 0 or starts.stride(0) == 1), \
+            assert starts.dtype is torch.int32 and starts.shape == (n + 1,) and (n == 0 or starts.stride(0) == 1), \
                 f"starts must be ({n + 1},) int32, contiguous, got {tuple(starts.shape)} {starts.dtype}"
-            self._check_device(starts, "starts")
-        out = None
+            if starts.get_device() != self._device:
+                self._wrong_device(starts, "starts")
+            starts_ptr = starts.data_ptr()
+        out, qp, qo, qs, hq, turn = None, 0, 0, (0, 0), 0, (0, 0, 0, 1.0)
+        if rotary is not None:
+            assert rotary.rotary_dim <= self.head_dim, f"rotary_dim {rotary.rotary_dim} exceeds head_dim {self.head_dim}"
+            if rotary._device != self._device:
+                self._wrong_device(rotary.inv_freq, "inv_freq")
+            turn = (rotary.inv_freq.data_ptr(), rotary.rotary_dim, rotary.interleaved, rotary.factor)
         if q is not None:
             assert rotary is not None, "q is only rotated: pass rotary with it"
             q = self._check_heads(q, "q", rows, None)
-            assert q.shape[1] > 0, "q has no heads"
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        turn = (0, 0, 0, 1.0)
-        if rotary is not None:
-            assert rotary.rotary_dim <= self.head_dim, f"rotary_dim {rotary.rotary_dim} exceeds head_dim {self.head_dim}"
-            self._check_device(rotary.inv_freq, "inv_freq")
-            turn = (rotary.inv_freq.data_ptr(), rotary.rotary_dim, rotary.interleaved, rotary.factor)
+            hq = q.shape[1]
+            assert hq > 0, "q has no heads"
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            qp, qo, qs = q.data_ptr(), out.data_ptr(), q.stride()[:2]
         if rows == 0:
             return out
         if n == 0:
             return None if out is None else out.zero_()
-        qs = (0, 0) if q is None else q.stride()[:2]
-        with torch.cuda.device(k.device):
-            _native.check(_native.lib().da_append_pages(_native.PACK_APPEND(
-                0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q is None else out.data_ptr(),
-                *qs, *k.stride()[:2], *v.stride()[:2], self.pages.data_ptr(), *self._strides, self.page_size, self.n_pages,
-                page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-                0 if starts is None else starts.data_ptr(), n, rows, *turn, 0 if q is None else q.shape[1], self.n_kv_heads,
-                self.head_dim, _native.dtype_code(k.dtype), self.status.data_ptr(), _native.stream_ptr())), "da_append_pages")
+        _native.launch(_native.lib().da_append_pages, _native.PACK_APPEND(
+            qp, k.data_ptr(), v.data_ptr(), qo, *qs, *k.stride()[:2], *v.stride()[:2], *self._pool, page_table.data_ptr(),
+            table_stride, columns, lengths.data_ptr(), starts_ptr, n, rows, *turn, hq, self.n_kv_heads, self.head_dim,
+            self._dtype_code, self.status.data_ptr(), _native.stream_of(self._device)), self._device, "da_append_pages")
         return out
 
     def attend(self, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *, window: int = 0,
@@ -144,31 +154,34 @@ class PagedKVCache:
         KV head h // (Hq / n_kv_heads)), over the first lengths[b] tokens of its sequence, or the last `window` of them.
         Logits are scaled by `scale` (default 1 / sqrt(D)).  Returns (n_sequences, Hq, D); with `return_lse` also the float32
         log-sum-exp of the scaled logits (n_sequences, Hq).  A sequence of length 0 gives zeros and -inf."""
-        n = self._check_table(page_table, lengths)
+        n, columns, table_stride = self._check_table(page_table, lengths)
         q = self._check_heads(q, "q", n, None)
         hq = q.shape[1]
-        assert hq > 0 and hq % self.n_kv_heads == 0, f"{hq} query heads do not divide among {self.n_kv_heads} KV heads"
         rep = hq // self.n_kv_heads
+        assert rep > 0 and hq == rep * self.n_kv_heads, f"{hq} query heads do not divide among {self.n_kv_heads} KV heads"
         assert window >= 0, f"window must not be negative, got {window}"
-        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        piece = 16 // q.element_size()
-        if q.data_ptr() % 16 or any(s % piece for s in q.stride()[:2]):
+        strides = q.stride()
+        if q.data_ptr() % 16 or strides[0] % self._piece or strides[1] % self._piece:
             q = q.clone(memory_format=torch.contiguous_format)
-        with torch.cuda.device(q.device):
-            out = torch.empty(n, hq, self.head_dim, dtype=q.dtype, device=q.device)
-            lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
-            if n:
-                dtype = _native.dtype_code(q.dtype)
-                lib = _native.lib()
-                # scratch of this call alone: two captured steps, or two streams, never share it
-                size = lib.da_paged_attention_workspace_bytes(rep, self.head_dim, dtype)
-                workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
-                _native.check(lib.da_paged_attention(_native.PACK_ATTEND(
-                    q.data_ptr(), *q.stride()[:2], self.pages.data_ptr(), *self._strides, self.page_size, self.n_pages,
-                    page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(), n, window, scale,
-                    out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size, self.status.data_ptr(),
-                    self.n_kv_heads, rep, self.head_dim, dtype, _native.stream_ptr())), "da_paged_attention")
+            strides = q.stride()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
+        if n:
+            # scratch of this call alone: two captured steps, or two streams, never share it
+            size, like = self._scratch.get(rep) or self._scratch_like(rep)
+            scratch = torch.empty_like(like)
+            _native.launch(_native.lib().da_paged_attention, _native.PACK_ATTEND(
+                q.data_ptr(), strides[0], strides[1], *self._pool, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
+                n, window, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), out.data_ptr(),
+                0 if lse is None else lse.data_ptr(), scratch.data_ptr(), size, self.status.data_ptr(), self.n_kv_heads, rep,
+                self.head_dim, self._dtype_code, _native.stream_of(self._device)), self._device, "da_paged_attention")
         return (out, lse) if return_lse else out
+
+    def _scratch_like(self, rep: int):
+        """Bytes of scratch for `rep` query heads per KV head, and a tensor of that many elements (one byte of memory) to make it like"""
+        size = _native.lib().da_paged_attention_workspace_bytes(rep, self.head_dim, self._dtype_code)
+        entry = self._scratch[rep] = (size, torch.empty(1, dtype=torch.uint8, device=self.pages.device).expand(max(size, 16)))
+        return entry
 
     def check_status(self) -> None:
         """Synchronises; raises if any call on this pool flagged a problem."""

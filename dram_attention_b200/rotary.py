@@ -80,64 +80,65 @@ class Rotary:
             f"inv_freq must be a float32 vector, got {tuple(inv_freq.shape)} {inv_freq.dtype}"
         _native.lib()
         self.inv_freq = inv_freq.detach().contiguous()
+        self.rotary_dim = 2 * inv_freq.numel()
         self.factor = float(factor)
         self.interleaved = bool(interleaved)
-
-    @property
-    def rotary_dim(self) -> int:
-        return 2 * self.inv_freq.numel()
+        self._device = inv_freq.get_device()
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
         """q (s, Hq, D) or (b, s, Hq, D), k the same with its own number of heads; positions int32 or int64, (s,) or (b, s),
         magnitudes below 2^31.  Channels from rotary_dim on pass unchanged.  Returns the rotated pair (new tensors);
-        differentiable in q and k."""
-        assert q.dim() in (3, 4) and k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == q.shape[-1], \
+        differentiable in q and k.  (As with every differentiable call: let go of results of eager calls on the same leaves
+        before a call and its backward pass are captured into a graph, torch ties the leaves' gradients to the eager stream.)"""
+        lead, device, rotary_dim = q.shape[:-2], q.get_device(), self.rotary_dim
+        assert 1 <= len(lead) <= 2 and k.shape[:-2] == lead and k.shape[-1] == q.shape[-1], \
             f"q (..., heads, D) and k (..., heads, D) do not go together: {tuple(q.shape)}, {tuple(k.shape)}"
-        _native.require_cuda(q, "q")
+        if device < 0:
+            _native.require_cuda(q, "q")
         assert k.dtype == q.dtype, "q and k must have the same dtype"
-        _native.dtype_code(q.dtype)
-        assert self.rotary_dim <= q.shape[-1] <= 512, \
-            f"head_dim must lie between rotary_dim ({self.rotary_dim}) and 512, got {q.shape[-1]}"
-        assert positions.dtype in (torch.int32, torch.int64), f"positions must be int32 or int64, got {positions.dtype}"
-        lead = q.shape[:-2]
-        assert positions.shape == lead or positions.shape == lead[-1:], \
-            f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}"
-        for t, name in ((k, "k"), (positions, "positions"), (self.inv_freq, "inv_freq")):
-            assert t.device == q.device, f"{name} must be on the device of q ({q.device}), got {t.device}"
-        positions = positions.expand(lead)
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        assert rotary_dim <= q.shape[-1] <= 512, \
+            f"head_dim must lie between rotary_dim ({rotary_dim}) and 512, got {q.shape[-1]}"
+        assert positions.dtype in _POSITION_TYPES, f"positions must be int32 or int64, got {positions.dtype}"
+        if positions.shape != lead:
+            assert positions.shape == lead[-1:], \
+                f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}"
+            positions = positions.expand(lead)
+        assert k.get_device() == positions.get_device() == self._device == device, \
+            f"k ({k.device}), positions ({positions.device}) and inv_freq ({self.inv_freq.device}) must be on the device of q ({q.device})"
+        if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
             return _Rotate.apply(q, k, positions, self.inv_freq, self.factor, self.interleaved, False)
         return _rotate(q, k, positions, self.inv_freq, self.factor, self.interleaved, False)
+
+
+_POSITION_TYPES = (torch.int32, torch.int64)
+_NOTHING = (0, 0, (0, 0, 0), 0)
+
+
+def _side(t: torch.Tensor):
+    """The output for q or k and what the call is told of the pair: addresses, strides (batch, token, head), heads"""
+    strides = t.stride()
+    if strides[-1] != 1:
+        t = t.contiguous()
+        strides = t.stride()
+    out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    # (a tensor without elements takes part in the call no more than None does: its address is null)
+    return out, (t.data_ptr(), out.data_ptr(), strides[:3] if len(strides) == 4 else (0, strides[0], strides[1]), t.shape[-2])
 
 
 def _rotate(q, k, positions, inv_freq, factor, interleaved, transposed):
     """Enqueue da_rotate; q or k may be None.  Returns new tensors."""
     x = k if q is None else q
-    lead, d = x.shape[:-2], x.shape[-1]
-    out, fields = [], []
-    for t in (q, k):
-        if t is None:
-            out.append(None)
-            fields.append((0, 0, (0, 0, 0), 0))
-            continue
-        t = t if t.stride(-1) == 1 else t.contiguous()
-        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        s = t.stride()
-        # (a tensor without elements takes part in the call no more than None does)
-        present = o.numel() > 0
-        out.append(o)
-        fields.append((t.data_ptr() if present else 0, o.data_ptr() if present else 0,
-                       (s[0] if len(lead) == 2 else 0, s[-3], s[-2]), t.shape[-2]))
-    (qp, qo, qs, hq), (kp, ko, ks, hk) = fields
-    if not (qp or kp):
-        return tuple(out)
-    ps = positions.stride()
-    with torch.cuda.device(x.device):
-        _native.check(_native.lib().da_rotate(_native.PACK_ROTATE(
-            qp, kp, qo, ko, *qs, *ks, positions.data_ptr(), positions.dtype == torch.int64, ps[0] if len(lead) == 2 else 0, ps[-1],
-            inv_freq.data_ptr(), 2 * inv_freq.numel(), interleaved, transposed, factor,
-            lead[0] if len(lead) == 2 else 1, lead[-1], hq, hk, d, _native.dtype_code(x.dtype), _native.stream_ptr())), "da_rotate")
-    return tuple(out)
+    q2, (qp, qo, qs, hq) = (None, _NOTHING) if q is None else _side(q)
+    k2, (kp, ko, ks, hk) = (None, _NOTHING) if k is None else _side(k)
+    if not qo and not ko:
+        return q2, k2
+    shape, device, ps = x.shape, x.get_device(), positions.stride()
+    batch, ps = (shape[0], ps) if len(shape) == 4 else (1, (0, ps[0]))
+    _native.launch(_native.lib().da_rotate, _native.PACK_ROTATE(
+        qp if qo else 0, kp if ko else 0, qo, ko, *qs, *ks, positions.data_ptr(), positions.dtype is torch.int64, *ps,
+        inv_freq.data_ptr(), 2 * inv_freq.shape[0], interleaved, transposed, factor, batch, shape[-3], hq, hk, shape[-1],
+        _native.dtype_code(x.dtype), _native.stream_of(device)), device, "da_rotate")
+    return q2, k2
 
 
 class _Rotate(torch.autograd.Function):
