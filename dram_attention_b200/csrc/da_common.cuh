@@ -44,6 +44,17 @@ template <> __device__ __forceinline__ void unpack2<__half>(uint32_t w, float &l
     hi = f.y;
 }
 
+// The other way: two floats rounded into one word.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+
 // Convert N consecutive elements, given as raw 32-bit words, to float.
 template <typename T, int N> struct Unpack {
     static constexpr int kWords = N * (int)sizeof(T) / 4;

@@ -8,16 +8,17 @@
 // rounded: at position 1 000 000 a 32-bit product is off by up to 0.03 rad, this one by 3e-8 at any position.  Products and
 // sums are 32-bit, the result is rounded once to the element type.
 //
-// Bound by memory: a token of 32 + 8 heads of 128 bf16 channels is 10 KB in and 10 KB out against 64 angles.  One CTA per
-// token (few tokens: several, each with some of the heads): the angles are made once per CTA and kept in shared memory, while
-// the rows, already requested, are on their way; a thread keeps its place in the head and goes from row to row.
+// Bound by memory: a token of 32 + 8 heads of 128 bf16 channels is 10 KB in and 10 KB out against 64 angles.  What stands in the
+// way is the number of instructions, so a thread keeps its place: one column of up to four neighbouring heads, for several
+// tokens in turn.  Addresses are then sums, the sines and cosines of a token are read once for four rows, and the
+// angles, positions and (append) places in the pool are made once per token of the block, while the first rows are on their way.
 
 #include "da_common.cuh"
 
 namespace da {
 
-constexpr int kRotateThreads = 256;   // about; the block is a whole number of rows
-constexpr int kRotateUnroll = 2;      // rows a thread has under way
+constexpr int kRotateRows = 4;        // most heads of a thread
+constexpr int kRotateTokens = 64;     // most tokens of a block
 
 struct RotateParams {
     // sources: queries, keys and (append) values; strides in elements
@@ -25,14 +26,17 @@ struct RotateParams {
     long long src_batch[3], src_token[3], src_head[3];
     int heads[3];
     void *dst[2];                     // rotated queries and keys, contiguous (append: queries only)
-    int n_tokens;                     // per batch entry (append: rows of the ragged batch)
+    int n_tokens;                     // per batch entry, as the sources see it (append: rows of the ragged batch)
+    int all_tokens;                   // of all batch entries
+    int rows_each;                    // heads of a thread
+    int rounds;                       // tokens of a thread
     int head_dim, rot_half;
     const float *inv_freq;
     float factor, sign;
     const void *positions;
     int positions_64;
+    int position_tokens;              // per batch entry, as the positions see it
     long long position_batch, position_token;
-    int rows_per_cta;
     // append
     void *pages;
     long long page_stride, page_head_stride;
@@ -56,30 +60,43 @@ __device__ __forceinline__ float2 cos_sin_turns(double turns) {
     return make_float2((quadrant == 1 || quadrant == 2) ? -a : a, quadrant >= 2 ? -b : b);
 }
 
+template <int BYTES> struct Words;
+template <> struct Words<16> { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<4> { using type = uint32_t; };
+template <> struct Words<2> { using type = unsigned short; };
+
+// V consecutive elements in one access.
 template <typename T, int V> struct Chunk {
-    static_assert(V * sizeof(T) == 16, "vectors are 16 bytes");
-    uint4 raw;
-    __device__ __forceinline__ void load(const T *p) { raw = __ldcs(reinterpret_cast<const uint4 *>(p)); }
-    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = raw; }
-    __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+    using Raw = typename Words<V * (int)sizeof(T)>::type;
+    Raw raw;
+    __device__ __forceinline__ void load(const T *p) { raw = __ldcs(reinterpret_cast<const Raw *>(p)); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<Raw *>(p) = raw; }
+    __device__ __forceinline__ void zero() { raw = Raw{}; }
     __device__ __forceinline__ void unpack(float (&x)[V]) const {
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        Unpack<T, V>::run(w, x);
+        union { Raw r; T t[V]; uint32_t w[V > 1 ? V * sizeof(T) / 4 : 1]; } u;
+        u.r = raw;
+        if constexpr (V == 1) {
+            x[0] = to_float(u.t[0]);
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = u.t[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) unpack2<T>(u.w[i], x[2 * i], x[2 * i + 1]);
+        }
     }
     __device__ __forceinline__ void pack(const float (&x)[V]) {
-        union { T t[V]; uint4 v; } u;
+        union { Raw r; T t[V]; uint32_t w[V > 1 ? V * sizeof(T) / 4 : 1]; } u;
+        if constexpr (V == 1 || sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) u.t[i] = from_float<T>(x[i]);
-        raw = u.v;
+            for (int i = 0; i < V; ++i) u.t[i] = from_float<T>(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) u.w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+        }
+        raw = u.r;
     }
-};
-template <typename T> struct Chunk<T, 1> {
-    T raw;
-    __device__ __forceinline__ void load(const T *p) { raw = *p; }
-    __device__ __forceinline__ void store(T *p) const { *p = raw; }
-    __device__ __forceinline__ void zero() { raw = from_float<T>(0.f); }
-    __device__ __forceinline__ void unpack(float (&x)[1]) const { x[0] = to_float(raw); }
-    __device__ __forceinline__ void pack(const float (&x)[1]) { raw = from_float<T>(x[0]); }
 };
 
 // (a, b) turned by (cos, sin)
@@ -130,145 +147,200 @@ __device__ __forceinline__ Place find_place(const RotateParams &p, int row) {
     return at;
 }
 
-// HALF: channel i is paired with channel i + rot / 2; otherwise with its neighbour.  A thread's task is its column of the
-// block: in front the tasks that rotate (both members' chunks of V channels; neighbours: one chunk that holds whole pairs, or
-// the two channels of a pair when V is 1), then those that copy a chunk behind the rotated part.
+// HALF: channel i is paired with channel i + rot / 2; otherwise with its neighbour.  A thread's column: in front those that
+// rotate (both members' chunks of V channels; neighbours: one chunk that holds whole pairs, or the two channels of a pair when
+// V is 1), then those that copy a chunk behind the rotated part.
 template <typename T, int V, bool HALF, bool PAGED>
-__global__ void __launch_bounds__(kRotateThreads * 2)
+__global__ void __launch_bounds__(512)
 rotate_kernel(const RotateParams p) {
-    constexpr bool kTwo = HALF || V == 1;         // a rotating task has two chunks
-    extern __shared__ float2 cos_sin[];           // [rot_half]
+    constexpr bool kTwo = HALF || V == 1;         // a rotating column has two chunks
+    constexpr int kPairs = kTwo ? V : V / 2;      // its pairs
+    extern __shared__ float2 cos_sin[];           // [tokens of the block][rot_half]
+    __shared__ long long sh_position[kRotateTokens];
+    __shared__ long long sh_place[PAGED ? kRotateTokens : 1];   // offset in the pool, -1: no page, -2: a row of no sequence
     griddep_wait();
     griddep_launch_dependents();
-    const int task = threadIdx.x, y = threadIdx.y;
+    const int column = threadIdx.x, z = threadIdx.z;
+    const int linear = (z * blockDim.y + threadIdx.y) * blockDim.x + column, threads = blockDim.x * blockDim.y * blockDim.z;
     const int n_turn = kTwo ? p.rot_half / V : (2 * p.rot_half + V - 1) / V;
-    const bool turns = task < n_turn;
-    const int at0 = turns ? (V == 1 && !HALF ? 2 * task : task * V)
-                          : (kTwo ? 2 * p.rot_half + (task - n_turn) * V : task * V);
-    const int at1 = HALF ? p.rot_half + task * V : at0 + 1;
-    const bool two = kTwo && turns;
+    const bool turns = column < n_turn, two = kTwo && turns;
+    const int at0 = turns ? (V == 1 && !HALF ? 2 * column : column * V)
+                          : (kTwo ? 2 * p.rot_half + (column - n_turn) * V : column * V);
+    const int at1 = HALF ? p.rot_half + column * V : at0 + 1;
 
-    const int row0 = blockIdx.y * p.rows_per_cta;
-    const int row_end = min(row0 + p.rows_per_cta, p.heads[0] + p.heads[1] + p.heads[2]);
-    const int token = blockIdx.x % p.n_tokens, batch = blockIdx.x / p.n_tokens;
-
-    Chunk<T, V> a[kRotateUnroll], b[kRotateUnroll];
-    auto request = [&](int base) {
+    // this thread's heads: `mine` of one kind from head0 on
+    int kind = 0, head0 = (blockIdx.y * blockDim.y + threadIdx.y) * p.rows_each;
 #pragma unroll
-        for (int i = 0; i < kRotateUnroll; ++i) {
-            const int r = base + i * blockDim.y;
-            if (r >= row_end) continue;
-            const int which = r < p.heads[0] ? 0 : (r < p.heads[0] + p.heads[1] ? 1 : 2);
-            const int head = which == 0 ? r : (which == 1 ? r - p.heads[0] : r - p.heads[0] - p.heads[1]);
-            const T *s = static_cast<const T *>(p.src[which]) + batch * p.src_batch[which] + token * p.src_token[which] +
-                         head * p.src_head[which];
-            a[i].load(s + at0);
-            if (two) b[i].load(s + at1);
+    for (int i = 0; i < 2; ++i) {
+        const int all = (p.heads[i] + p.rows_each - 1) / p.rows_each * p.rows_each;
+        if (kind == i && head0 >= all) head0 -= all, ++kind;
+    }
+    const int mine = min(p.rows_each, p.heads[kind] - head0);
+
+    const int per_block = blockDim.z * p.rounds;
+    const int first = blockIdx.x * per_block;
+    const int here = min(per_block, p.all_tokens - first);      // tokens of this block
+
+    const T *base = static_cast<const T *>(p.src[kind]) + head0 * p.src_head[kind];
+    const long long src_head = p.src_head[kind];
+    Chunk<T, V> a[kRotateRows], b[kRotateRows];
+    auto request = [&](int t) {
+        if (t >= here) return;
+        int batch = 0, token = first + t;
+        if (!PAGED && p.n_tokens != p.all_tokens) batch = token / p.n_tokens, token -= batch * p.n_tokens;
+        const T *s = base + (batch * p.src_batch[kind] + token * p.src_token[kind]);
+#pragma unroll
+        for (int i = 0; i < kRotateRows; ++i) {
+            if (i < mine) {
+                a[i].load(s + at0);
+                if (two) b[i].load(s + at1);
+            }
+            s += src_head;
         }
     };
-    request(row0 + y);
+    request(z);
 
-    // the token's position and its angles, while the rows are on their way
-    Place at = {0, -1, 0, true, 0};
-    if constexpr (PAGED) {
-        at = find_place(p, token);
-        if (at.status && blockIdx.y == 0 && task == 0 && y == 0) atomicOr(p.status, at.status);
-    } else {
-        const long long i = batch * p.position_batch + token * p.position_token;
-        at.position = p.positions_64 ? __ldg(static_cast<const long long *>(p.positions) + i)
-                                     : (long long)__ldg(static_cast<const int32_t *>(p.positions) + i);
+    // the tokens' positions and places, while the first rows are on their way
+    if (linear < here) {
+        const int t = first + linear;
+        if constexpr (PAGED) {
+            const Place at = find_place(p, t);
+            if (at.status && blockIdx.y == 0) atomicOr(p.status, at.status);
+            sh_position[linear] = at.position;
+            sh_place[linear] = !at.used ? -2 : (at.page < 0 ? -1 : at.page * p.page_stride + (long long)at.slot * 2 * p.head_dim);
+        } else {
+            const int n = t / p.position_tokens;
+            const long long i = n * p.position_batch + (t - n * p.position_tokens) * p.position_token;
+            sh_position[linear] = p.positions_64 ? __ldg(static_cast<const long long *>(p.positions) + i)
+                                                 : (long long)__ldg(static_cast<const int32_t *>(p.positions) + i);
+        }
     }
-    for (int i = y * blockDim.x + task; i < p.rot_half; i += blockDim.x * blockDim.y) {
-        const double per_turn = (double)__ldg(p.inv_freq + i) * 0.15915494309189535;   // 1 / 2 pi
-        float2 cs = cos_sin_turns((double)at.position * per_turn);
+    __syncthreads();
+    for (int i = linear; i < here * p.rot_half; i += threads) {
+        const int t = i / p.rot_half, pair = i - t * p.rot_half;
+        const double per_turn = (double)__ldg(p.inv_freq + pair) * 0.15915494309189535;   // 1 / 2 pi
+        const float2 cs = cos_sin_turns((double)sh_position[t] * per_turn);
         cos_sin[i] = make_float2(cs.x * p.factor, cs.y * p.factor * p.sign);
     }
     __syncthreads();
 
-    for (int base = row0 + y; base < row_end; base += kRotateUnroll * blockDim.y) {
-        if (base != row0 + y) request(base);
+    // a chunk that ends behind the rotated part: its last pairs are copied, not multiplied by 1 and 0
+    const int pairs = kTwo ? V : min(V / 2, p.rot_half - column * (V / 2));
+    const bool rotates = turns && kind != 2;
+    const bool to_pages = PAGED && kind != 0;
+    T *const out = to_pages ? static_cast<T *>(p.pages) + head0 * p.page_head_stride + (kind == 2 ? p.head_dim : 0)
+                            : static_cast<T *>(p.dst[kind < 2 ? kind : 0]) + ((long long)first * p.heads[kind] + head0) * p.head_dim;
+    const long long out_head = to_pages ? p.page_head_stride : p.head_dim;
+    for (int t = z; t < here; t += blockDim.z) {
+        const float2 *cs = cos_sin + t * p.rot_half + column * kPairs;
+        const long long place = PAGED ? sh_place[t] : 0;
+        T *d = out + (to_pages ? place : (long long)t * p.heads[kind] * p.head_dim);
+        if (rotates) {
+            float2 w[kPairs];
 #pragma unroll
-        for (int i = 0; i < kRotateUnroll; ++i) {
-            const int r = base + i * blockDim.y;
-            if (r >= row_end) continue;
-            const int which = r < p.heads[0] ? 0 : (r < p.heads[0] + p.heads[1] ? 1 : 2);
-            const int head = which == 0 ? r : (which == 1 ? r - p.heads[0] : r - p.heads[0] - p.heads[1]);
-            if (turns && which != 2) {
+            for (int j = 0; j < kPairs; ++j) w[j] = kTwo || j < pairs ? cs[j] : make_float2(1.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kRotateRows; ++i) {
+                if (i >= mine) continue;
                 float x[V];
                 a[i].unpack(x);
                 if constexpr (kTwo) {
-                    float z[V];
-                    b[i].unpack(z);
+                    float u[V];
+                    b[i].unpack(u);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) turn(x[j], z[j], cos_sin[task * V + j]);
-                    b[i].pack(z);
+                    for (int j = 0; j < V; ++j) turn(x[j], u[j], w[j]);
+                    b[i].pack(u);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {
-                        const int pair = task * (V / 2) + j;
-                        if (pair < p.rot_half) turn(x[2 * j], x[2 * j + 1], cos_sin[pair]);
-                    }
+                    for (int j = 0; j < V / 2; ++j)
+                        if (j < pairs) turn(x[2 * j], x[2 * j + 1], w[j]);
                 }
                 a[i].pack(x);
             }
-            T *d;
-            if (PAGED && which != 0) {
-                if (at.page < 0) continue;
-                d = static_cast<T *>(p.pages) + head * p.page_head_stride + at.page * p.page_stride +
-                    (long long)at.slot * 2 * p.head_dim + (which == 2 ? p.head_dim : 0);
-            } else {
-                d = static_cast<T *>(p.dst[which]) + ((long long)blockIdx.x * p.heads[which] + head) * p.head_dim;
-                if (PAGED && !at.used) {   // a row of no sequence
-                    a[i].zero();
-                    b[i].zero();
-                }
-            }
-            a[i].store(d + at0);
-            if (two) b[i].store(d + at1);
         }
+        if (PAGED && kind == 0 && place == -2) {
+#pragma unroll
+            for (int i = 0; i < kRotateRows; ++i) a[i].zero(), b[i].zero();
+        }
+        if (!to_pages || place >= 0) {
+#pragma unroll
+            for (int i = 0; i < kRotateRows; ++i) {
+                if (i < mine) {
+                    a[i].store(d + at0);
+                    if (two) b[i].store(d + at1);
+                }
+                d += out_head;
+            }
+        }
+        request(t + blockDim.z);
     }
 }
 
 template <typename T, int V, bool HALF, bool PAGED>
 static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     const int rot = 2 * p.rot_half, d = p.head_dim;
-    const int tasks = (HALF || V == 1) ? p.rot_half / V + (d - rot) / V : d / V;
-    const int rows = p.heads[0] + p.heads[1] + p.heads[2];
-    const long long tokens = (long long)n_batch * p.n_tokens;
-    // Few tokens: their rows are spread over as many CTAs as leave each at least two warps.
-    int per_cta = rows;
-    if (tokens < 148) {
-        const int least = (64 + tasks - 1) / tasks;
-        const int splits = (int)(148 / tokens);
-        per_cta = (rows + splits - 1) / splits;
-        if (per_cta < least) per_cta = least;
-        if (per_cta > rows) per_cta = rows;
+    const int columns = (HALF || V == 1) ? p.rot_half / V + (d - rot) / V : d / V;
+    p.all_tokens = n_batch * p.n_tokens;
+    auto threads_for = [&](int each) {
+        int y = 0;
+        for (int h : p.heads) y += (h + each - 1) / each;
+        return y;
+    };
+    // Many tokens: as many heads to a thread as leave fewest places empty, the larger number of two that do; few: one, so that
+    // every row sets out at once.
+    p.rows_each = 1;
+    if ((long long)p.all_tokens * threads_for(1) * columns > 148 * 1024) {
+        long long best = -1;
+        for (int each = kRotateRows; each >= 1; --each) {
+            const long long places = (long long)threads_for(each) * each;
+            if (best < 0 || places * 8 < best * 7) best = places, p.rows_each = each;
+        }
     }
-    p.rows_per_cta = per_cta;
-    const int splits = (rows + per_cta - 1) / per_cta;
-    // as many rows at a time as fill the block, evenly over the passes
-    int y = kRotateThreads / tasks;
+    // Whole tokens up to the size of a block.  Small blocks and one token per thread are fastest (32 768 tokens of 32 + 8 heads in
+    // halves: 105 us with blocks of 96 to 192 threads, 115 with 384; two tokens in turn 127), but for an append whose columns are one
+    // chunk: the look-up of the places is then worth sharing (32 768 tokens: 126 us with 384 threads and two tokens in turn,
+    // 136 with 128 and one).
+    constexpr bool kShare = PAGED && !HALF && V > 1;
+    constexpr int THREADS = kShare ? 384 : 128;
+    const int all_y = threads_for(p.rows_each);
+    int y = columns * all_y <= 192 ? all_y : THREADS / columns;   // (the angles of a token are made once, then)
     if (y < 1) y = 1;
-    const int passes = (per_cta + y - 1) / y;
-    y = (per_cta + passes - 1) / passes;
-    const cudaError_t e = launch_dependent(rotate_kernel<T, V, HALF, PAGED>, dim3((unsigned)tokens, splits), dim3(tasks, y),
-                                           p.rot_half * sizeof(float2), stream, p);
-    return (int)e;
+    const int blocks_y = (all_y + y - 1) / y;
+    y = (all_y + blocks_y - 1) / blocks_y;
+    int z = THREADS / (columns * y);
+    if (z > kRotateTokens / 2) z = kRotateTokens / 2;
+    while (z > 1 && p.all_tokens / z < 148) z >>= 1;
+    if (z < 1) z = 1;
+    const int rounds = kShare && p.all_tokens / z >= 2 * 8 * 148 ? 2 : 1;
+    p.rounds = rounds;
+    const int per_block = z * rounds;
+    return (int)launch_dependent(rotate_kernel<T, V, HALF, PAGED>, dim3((unsigned)(((long long)p.all_tokens + per_block - 1) / per_block), blocks_y),
+                                 dim3(columns, y, z), (size_t)per_block * p.rot_half * sizeof(float2), stream, p);
+}
+
+// V: the longest access that every row and (halves) the second half start on a multiple of, up to 16 bytes
+template <typename T, bool PAGED>
+static int rotate_by(const RotateParams &p, int n_batch, bool half, int v, cudaStream_t stream) {
+    constexpr int MOST = 16 / (int)sizeof(T);
+    if (v >= MOST) return half ? launch_rotate<T, MOST, true, PAGED>(p, n_batch, stream) : launch_rotate<T, MOST, false, PAGED>(p, n_batch, stream);
+    if (v >= 2) return half ? launch_rotate<T, 2, true, PAGED>(p, n_batch, stream) : launch_rotate<T, 2, false, PAGED>(p, n_batch, stream);
+    return half ? launch_rotate<T, 1, true, PAGED>(p, n_batch, stream) : launch_rotate<T, 1, false, PAGED>(p, n_batch, stream);
 }
 
 template <bool PAGED>
-static int rotate(const RotateParams &p, int n_batch, int dtype, bool half, bool vectors, cudaStream_t stream) {
+static int rotate(const RotateParams &p, int n_batch, int dtype, bool half, int v, cudaStream_t stream) {
     switch (dtype) {
-    case DA_F32:
-        if (vectors) return half ? launch_rotate<float, 4, true, PAGED>(p, n_batch, stream) : launch_rotate<float, 4, false, PAGED>(p, n_batch, stream);
-        return half ? launch_rotate<float, 1, true, PAGED>(p, n_batch, stream) : launch_rotate<float, 1, false, PAGED>(p, n_batch, stream);
-    case DA_F16:
-        if (vectors) return half ? launch_rotate<__half, 8, true, PAGED>(p, n_batch, stream) : launch_rotate<__half, 8, false, PAGED>(p, n_batch, stream);
-        return half ? launch_rotate<__half, 1, true, PAGED>(p, n_batch, stream) : launch_rotate<__half, 1, false, PAGED>(p, n_batch, stream);
-    default:
-        if (vectors) return half ? launch_rotate<__nv_bfloat16, 8, true, PAGED>(p, n_batch, stream) : launch_rotate<__nv_bfloat16, 8, false, PAGED>(p, n_batch, stream);
-        return half ? launch_rotate<__nv_bfloat16, 1, true, PAGED>(p, n_batch, stream) : launch_rotate<__nv_bfloat16, 1, false, PAGED>(p, n_batch, stream);
+    case DA_F32: return rotate_by<float, PAGED>(p, n_batch, half, v, stream);
+    case DA_F16: return rotate_by<__half, PAGED>(p, n_batch, half, v, stream);
+    default: return rotate_by<__nv_bfloat16, PAGED>(p, n_batch, half, v, stream);
     }
+}
+
+// Elements of the longest power of two up to 16 bytes that divides all of them: the addresses (bytes), the strides and sizes (elements).
+static int access_elements(uintptr_t bases, int64_t elements, int esize) {
+    int v = 16 / esize;
+    while (v > 1 && ((bases & (uintptr_t)(v * esize - 1)) || (elements & (v - 1)))) v >>= 1;
+    return v;
 }
 
 static bool small(int64_t v, int64_t lo, int64_t hi) { return v >= lo && v <= hi; }
@@ -283,7 +355,7 @@ extern "C" int da_rotate(const da_rotate_args *args) {
     if (!small(a.dtype, DA_F32, DA_BF16)) return DA_ERR_DTYPE;
     if (!small(a.n_batch, 1, 1 << 24) || !small(a.n_tokens, 1, 1 << 30) || a.n_batch * a.n_tokens > 0x7fffffff ||
         !small(a.head_dim, 2, 512) || !small(a.rotary_dim, 2, a.head_dim) || (a.rotary_dim & 1) ||
-        (a.q && !small(a.n_q_heads, 1, 1 << 16)) || (a.k && !small(a.n_kv_heads, 1, 1 << 16)))
+        (a.q && !small(a.n_q_heads, 1, 1 << 14)) || (a.k && !small(a.n_kv_heads, 1, 1 << 14)))
         return DA_ERR_SHAPE;
     const int esize = a.dtype == DA_F32 ? 4 : 2;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
@@ -304,16 +376,19 @@ extern "C" int da_rotate(const da_rotate_args *args) {
         p.heads[i] = (int)heads[i];
     }
     p.dst[0] = a.q_out, p.dst[1] = a.k_out;
-    p.n_tokens = (int)a.n_tokens;
+    p.n_tokens = p.position_tokens = (int)a.n_tokens;
+    int n_batch = (int)a.n_batch;
+    // batch entries that follow one another as tokens do are one sequence of tokens
+    bool joined = true;
+    for (int i = 0; i < 2; ++i) joined = joined && (!src[i] || p.src_batch[i] == p.src_token[i] * a.n_tokens);
+    if (joined) p.n_tokens *= n_batch, n_batch = 1;
     p.head_dim = (int)a.head_dim, p.rot_half = (int)a.rotary_dim / 2;
     p.inv_freq = a.inv_freq, p.factor = (float)a.factor, p.sign = a.transposed ? -1.f : 1.f;
     p.positions = a.positions, p.positions_64 = a.positions_64 != 0;
     p.position_batch = a.position_strides[0], p.position_token = a.position_strides[1];
-    // 16-byte pieces, when every row and (halves) the second half start on such a boundary; otherwise channel by channel
-    const int v = 16 / esize;
     const bool half = a.interleaved == 0;
-    const bool vectors = !(bases & 15) && strides % v == 0 && a.head_dim % v == 0 && (!half || (a.rotary_dim / 2) % v == 0);
-    return rotate<false>(p, (int)a.n_batch, (int)a.dtype, half, vectors, static_cast<cudaStream_t>(a.stream));
+    const int v = access_elements(bases, strides | a.head_dim | (half ? p.rot_half : 0), esize);
+    return rotate<false>(p, n_batch, (int)a.dtype, half, v, static_cast<cudaStream_t>(a.stream));
 }
 
 extern "C" int da_append_pages(const da_append_pages_args *args) {
@@ -324,7 +399,7 @@ extern "C" int da_append_pages(const da_append_pages_args *args) {
         return DA_ERR_NULL;
     if (!small(a.dtype, DA_F32, DA_BF16)) return DA_ERR_DTYPE;
     if (!small(a.n_rows, 1, 1 << 30) || !small(a.n_sequences, 1, 1 << 30) || (!a.starts && a.n_rows != a.n_sequences) ||
-        !small(a.head_dim, 2, 512) || (a.q && !small(a.n_q_heads, 1, 1 << 16)) || !small(a.n_kv_heads, 1, 1 << 16) ||
+        !small(a.head_dim, 2, 512) || (a.q && !small(a.n_q_heads, 1, 1 << 14)) || !small(a.n_kv_heads, 1, 1 << 14) ||
         !small(a.page_size, 1, 1 << 20) || !small(a.n_pages, 1, 0x7fffffff) || !small(a.table_columns, 1, 0x7fffffff) ||
         a.table_columns * a.page_size > 0x7fffff00 ||
         (a.inv_freq && (!small(a.rotary_dim, 2, a.head_dim) || (a.rotary_dim & 1))))
@@ -357,8 +432,7 @@ extern "C" int da_append_pages(const da_append_pages_args *args) {
     p.table = a.page_table, p.table_stride = a.table_stride, p.table_cols = (int)a.table_columns;
     p.lengths = a.lengths, p.starts = a.starts, p.n_sequences = (int)a.n_sequences;
     p.status = a.status;
-    const int v = 16 / esize;
     const bool half = a.interleaved == 0;
-    const bool vectors = !(bases & 15) && strides % v == 0 && a.head_dim % v == 0 && (!half || p.rot_half % v == 0);
-    return rotate<true>(p, 1, (int)a.dtype, half, vectors, static_cast<cudaStream_t>(a.stream));
+    const int v = access_elements(bases, strides | a.head_dim | (half ? p.rot_half : 0), esize);
+    return rotate<true>(p, 1, (int)a.dtype, half, v, static_cast<cudaStream_t>(a.stream));
 }
