@@ -24,8 +24,11 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParam
     const Totals units = total_units(p, b, lane);
     const int length = __ldg(p.lengths + b);
     const int mine = span_of(p, length).units;
-    const long long begin = units.before + (long long)(item % per) * mine;
-    const int ctas = paged_ctas(p, units.all, kPagedCtas);
+    const long long begin = units.before * per + (long long)(item % per) * mine;
+    const Deal deal(units.all * per);
+    int c0 = 0, c1 = 0;
+    if (mine) c0 = deal.cta_of(begin), c1 = deal.cta_of(begin + mine - 1);
+
     griddep_wait();
     griddep_launch_dependents();
     if (blockIdx.y == 0 && threadIdx.x == 0 && item % per == 0 && (length < 0 || length > p.capacity)) atomicOr(p.status, DA_STATUS_BAD_POSITION);
@@ -38,7 +41,6 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParam
         }
         return;
     }
-    const int c0 = cta_of(units.all, ctas, begin), c1 = cta_of(units.all, ctas, begin + mine - 1);
     if (c0 == c1) return;                          // one CTA had all of it
 
     PartialSum x[NV];
@@ -173,7 +175,6 @@ extern "C" int da_paged_attention(const da_paged_attention_args *args) {
     if (a.n_sequences * a.n_kv_heads * p.groups > 0x7fffffff) return DA_ERR_SHAPE;
     p.cta_partials = static_cast<float *>(a.workspace);
     p.warp_partials = p.cta_partials + (size_t)kPagedCtas * 2 * p.group_rows * (a.head_dim + 4);
-    p.min_units = kPagedMaxWarps;
     p.scale_log2 = (float)(a.scale * 1.4426950408889634);
     cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
     cudaError_t e;

@@ -25,6 +25,7 @@ namespace da {
 
 constexpr int kPagedUnit = 16;        // tokens
 constexpr int kPagedCtas = 148;       // one per SM
+constexpr int kPagedMinUnits = 8;     // fewer are not worth a CTA of their own: a unit for every warp
 
 struct PagedParams {
     const unsigned char *q;
@@ -45,7 +46,6 @@ struct PagedParams {
     float *cta_partials;              // [CTA][2][group_rows][D + 4]
     int32_t *status;
     int n_kv_heads, rep, groups, group_rows;   // query rows of a KV head, in groups of at most group_rows
-    int min_units;                    // fewer units than this are not worth a CTA of their own
     float scale_log2;
 };
 
@@ -63,31 +63,25 @@ __device__ __forceinline__ Span span_of(const PagedParams &p, int length) {
     return s;
 }
 
-__device__ __forceinline__ long long shfl_64(long long v, int from) {
-    const int lo = __shfl_sync(DA_FULL_MASK, (int)(v & 0xffffffff), from);
-    const int hi = __shfl_sync(DA_FULL_MASK, (int)(v >> 32), from);
-    return ((long long)hi << 32) | (unsigned)lo;
-}
-// (a 64-bit division takes some hundred instructions; nearly every line is shorter than 2^32 / 148 units)
-__device__ __forceinline__ long long divide(long long n, long long d) {
-    if (((n | d) >> 32) == 0) return (long long)((uint32_t)n / (uint32_t)d);
+// (a 64-bit division takes some hundred instructions; nearly every line is shorter than 2^32 units)
+__device__ __forceinline__ long long divide(long long n, int d) {
+    if ((n >> 32) == 0) return (long long)((uint32_t)n / (uint32_t)d);
     return n / d;
 }
 
-// Units per lane and per (head, group) of 32 sequences from b0 on, and their inclusive sums.
-__device__ __forceinline__ long long scan_units(const PagedParams &p, int b0, int lane, int &mine) {
+// Units per (head, group) of 32 sequences from b0 on, one per lane, and their inclusive sums (below 2^32: 32 times 2^27).
+__device__ __forceinline__ uint32_t scan_units(const PagedParams &p, int b0, int lane, uint32_t &mine) {
     mine = b0 + lane < p.n_sequences ? span_of(p, __ldg(p.lengths + b0 + lane)).units : 0;
-    long long sum = mine;
+    uint32_t sum = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int lo = __shfl_up_sync(DA_FULL_MASK, (int)(sum & 0xffffffff), off);
-        const int hi = __shfl_up_sync(DA_FULL_MASK, (int)(sum >> 32), off);
-        if (lane >= off) sum += ((long long)hi << 32) | (unsigned)lo;
+        const uint32_t v = __shfl_up_sync(DA_FULL_MASK, sum, off);
+        if (lane >= off) sum += v;
     }
     return sum;
 }
 
-// Units of the whole launch, and of the sequences in front of `before` (all warps of a CTA compute the same).
+// Units per (head, group) of all sequences, and of those in front of `before`.
 struct Totals {
     long long all, before;
 };
@@ -103,19 +97,26 @@ __device__ __forceinline__ Totals total_units(const PagedParams &p, int before, 
         all += __shfl_xor_sync(DA_FULL_MASK, all, off);
         front += __shfl_xor_sync(DA_FULL_MASK, front, off);
     }
-    const int per = p.n_kv_heads * p.groups;
-    return {all * per, front * per};
+    return {all, front};
 }
 
-// How the line is dealt out.  CTA c has the units [c * total / ctas, (c + 1) * total / ctas).
-__device__ __forceinline__ int paged_ctas(const PagedParams &p, long long total, int most) {
-    const long long want = divide(total + p.min_units - 1, p.min_units);
-    return (int)(want < most ? want : most);
-}
-__device__ __forceinline__ long long cta_begin(long long total, int ctas, int c) { return divide(total * c, ctas); }
-__device__ __forceinline__ int cta_of(long long total, int ctas, long long unit) {
-    return (int)divide((unit + 1) * ctas - 1, total);
-}
+// How the line is dealt out: to as many CTAs as get kPagedMinUnits each, up to kPagedCtas, the first `more` of them one unit more.
+struct Deal {
+    int ctas, more;
+    long long each;
+    __device__ __forceinline__ explicit Deal(long long total) {
+        const long long want = (total + kPagedMinUnits - 1) / kPagedMinUnits;
+        ctas = (int)(want < kPagedCtas ? want : kPagedCtas);
+        each = ctas ? divide(total, ctas) : 0;
+        more = (int)(total - each * ctas);
+    }
+    __device__ __forceinline__ long long begin(int c) const { return each * c + min(c, more); }
+    __device__ __forceinline__ int cta_of(long long unit) const {
+        const long long long_part = (each + 1) * more;
+        if (unit < long_part) return (int)(unit / (each + 1));
+        return more + (int)((unit - long_part) / each);
+    }
+};
 
 template <int D> struct PagedRow { static constexpr int kWidth = D + 4; };   // accumulator, maximum, weight sum, padding
 
@@ -143,22 +144,20 @@ struct Cursor {
         }
         u = s.u0;
     }
-    // to unit `at` of the line, which has `total`; `first`, `first_sum` = scan_units of the first 32 sequences
-    __device__ __forceinline__ void seek(const PagedParams &p, long long at, int lane, int first, long long first_sum) {
+    // to unit `at` of the line; mine, sum: scan_units of the first 32 sequences
+    __device__ __forceinline__ void seek(const PagedParams &p, long long at, int lane, uint32_t mine, uint32_t sum) {
         const int per = p.n_kv_heads * p.groups;
-        long long front = 0, sum = first_sum;
-        int mine = first;
-        for (int b0 = 0;; b0 += 32) {
-            const unsigned past = __ballot_sync(DA_FULL_MASK, (front + sum) * per > at);
-            if (past || b0 + 32 >= p.n_sequences) {
-                const int l = past ? __ffs(past) - 1 : 31;
-                enter(p, min(b0 + l, p.n_sequences - 1));
-                front += shfl_64(sum - mine, l);
-                break;
-            }
-            front += shfl_64(sum, 31);
-            sum = scan_units(p, b0 + 32, lane, mine);
+        long long front = 0;
+        int b0 = 0;
+        unsigned past;
+        while ((past = __ballot_sync(DA_FULL_MASK, (front + sum) * per > at)) == 0 && b0 + 32 < p.n_sequences) {
+            front += __shfl_sync(DA_FULL_MASK, sum, 31);
+            b0 += 32;
+            sum = scan_units(p, b0, lane, mine);
         }
+        const int l = past ? __ffs(past) - 1 : 0;
+        front += __shfl_sync(DA_FULL_MASK, sum - mine, l);
+        enter(p, min(b0 + l, p.n_sequences - 1));
         const long long inside = at - front * per;
         const int item = (int)divide(inside, max(s.units, 1));
         head = item / p.groups;
@@ -230,7 +229,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     // before (2 w, in global memory: the ring is busy), and its last one (2 w + 1, in its ring).
     __shared__ int part_item[2 * WARPS];           // -1: none
     __shared__ int part_flags[2 * WARPS];          // 1: the item begins in the warp's stretch, 2: it ends there
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
     if (lane == 0) {
 #pragma unroll
@@ -243,15 +242,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     griddep_launch_dependents();
 
     // ---- this warp's stretch ------------------------------------------------------------
-    int first;
-    const long long first_sum = scan_units(p, 0, lane, first);
-    const long long total = p.n_sequences <= 32 ? shfl_64(first_sum, 31) * (p.n_kv_heads * p.groups) : total_units(p, 0, lane).all;
-    const int ctas = paged_ctas(p, total, gridDim.x);
-    if ((int)blockIdx.x >= ctas) return;
-    const long long lo = cta_begin(total, ctas, blockIdx.x);
-    const int mine = (int)(cta_begin(total, ctas, blockIdx.x + 1) - lo);
-    const int skip = (int)divide((long long)mine * warp, WARPS);
-    const int count = (int)divide((long long)mine * (warp + 1), WARPS) - skip;
+    uint32_t first;
+    const uint32_t first_sum = scan_units(p, 0, lane, first);
+    const long long total = p.n_sequences <= 32 ? (long long)__shfl_sync(DA_FULL_MASK, first_sum, 31) : total_units(p, 0, lane).all;
+    const Deal deal(total * (p.n_kv_heads * p.groups));
+    if ((int)blockIdx.x >= deal.ctas) return;
+    const long long lo = deal.begin(blockIdx.x);
+    const int mine = (int)deal.each + ((int)blockIdx.x < deal.more), spare = mine % WARPS;
+    const int skip = mine / WARPS * warp + min(warp, spare);
+    const int count = mine / WARPS + (warp < spare);
     unsigned char *ring = smem + (size_t)warp * STAGES * STAGEB;
 
     if (count > 0) {
@@ -382,7 +381,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     const int n_items = __popc(leads);
     const int tasks = p.group_rows * COLS;
     int at_item = 0;                               // leads: from this item on
-    for (int t = tid; t < n_items * tasks; t += WARPS * 32) {
+    for (int t = threadIdx.x; t < n_items * tasks; t += WARPS * 32) {
         const int g = t / tasks, e = t - g * tasks;
         const int r = e / COLS, c = e - r * COLS;
         for (; at_item < g; ++at_item) leads &= leads - 1;
