@@ -281,6 +281,15 @@ __device__ __forceinline__ void bulk_copy_g2s(void *dst_smem, const void *src_gm
 }
 
 
+// True in one lane of a converged warp.  Measured against a comparison of the lane number in front of the tensor-core and
+// copy instructions of the prefill (16384 tokens x 32 heads): 1850 us, with this and a warp number read from one lane 1765.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+
 // Brings `bytes` at `src` into L2 (address and size multiples of 16).
 __device__ __forceinline__ void bulk_prefetch_l2(const void *src, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");

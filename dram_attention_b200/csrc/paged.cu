@@ -167,6 +167,7 @@ extern "C" int da_paged_attention(const da_paged_attention_args *args) {
     while ((1 << l) < p.page_size) ++l;
     p.page_mul = (uint32_t)((1ull << (31 + l)) / (unsigned)p.page_size + 1);
     p.page_shift = 31 + l;
+    p.whole = p.page_size % kPagedUnit == 0;
     p.lengths = a.lengths, p.n_sequences = (int)a.n_sequences, p.window = (int)a.window;
     p.out = static_cast<unsigned char *>(a.out), p.lse = a.lse, p.status = a.status;
     p.n_kv_heads = (int)a.n_kv_heads, p.rep = (int)a.rep;

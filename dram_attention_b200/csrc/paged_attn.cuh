@@ -11,7 +11,10 @@
 // nothing about them has to be known on the host: every warp finds its place from the lengths itself, so a captured launch
 // stays right while the sequences grow.  A warp walks its stretch with a private ring of stages (one mbarrier each) that
 // bulk copies (TMA) fill, one per token: its key and value rows are contiguous in the page.  The ring runs on across the
-// borders of items; there is no barrier of the CTA until its stretch is done.
+// borders of items; there is no barrier of the CTA until its stretch is done.  Where a unit lies in one page a single elected lane
+// issues its copies: a bulk copy takes its operands from the warp, so one per lane is a loop over the lanes (60 sequences of 3000
+// tokens, 64 channels: 76 us, elected 64).  16-byte asynchronous copies of all lanes need fewer instructions still but
+// bring in less (64 sequences of 5000 tokens, 128 channels: 221 us against 197).
 //
 // An item that lies in one warp's stretch is written by the warp.  One that crosses warps is put together by the CTA from the
 // warps' partial results (row maximum, weight sum, accumulator: float32), and one that crosses CTAs by a second,
@@ -38,6 +41,7 @@ struct PagedParams {
     int capacity;                     // tokens a row of the table has room for
     uint32_t page_mul;                // t / page_size = (t * page_mul) >> page_shift
     int page_shift;
+    int whole;                        // a unit lies in one page: page_size is a multiple of 16
     const int32_t *lengths;
     int n_sequences, window;
     unsigned char *out;
@@ -125,11 +129,13 @@ struct Cursor {
     int b, head, group;               // the item
     int u, end;                       // unit inside the sequence, and the first behind its last
     Span s;
+    const int32_t *row;               // the sequence's pages
     __device__ __forceinline__ int id(const PagedParams &p) const { return (b * p.n_kv_heads + head) * p.groups + group; }
     __device__ __forceinline__ void enter(const PagedParams &p, int sequence) {
         b = sequence;
         s = span_of(p, __ldg(p.lengths + b));
         end = s.u0 + s.units;
+        row = p.table + b * p.table_stride;
     }
     // to the next unit of the line (there is one)
     __device__ __forceinline__ void next(const PagedParams &p) {
@@ -259,36 +265,56 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
         Cursor at = ahead;
         bool begins = at.u == at.s.u0;
 
-        // A lane's token of the unit to be requested next: its page (looked up one unit ahead), then its address.
+        // The unit to be requested next: its tokens that there are, and its page (pages not whole: each lane's token's), looked
+        // up one unit ahead; then where it lies.
         int page, slot;
+        uint32_t there;
         auto look_up = [&](const Cursor &c) {
-            const int t = c.u * kPagedUnit + lane;
-            page = -2;                             // no such token
-            slot = 0;
-            if (lane < kPagedUnit && t >= c.s.first && t < c.s.n) {
-                const int column = (int)(((unsigned long long)(unsigned)t * p.page_mul) >> p.page_shift);
-                slot = t - column * p.page_size;
-                page = __ldg(p.table + c.b * p.table_stride + column);
-                if (page < 0 || page >= p.n_pages) page = -1;
-            }
+            const int t0 = c.u * kPagedUnit, t = p.whole ? t0 : t0 + (lane & 15);
+            const int from = max(c.s.first - t0, 0), to = min(c.s.n - t0, kPagedUnit);
+            there = (0xffffu >> (kPagedUnit - to)) & (0xffffu << from);
+            const int column = (int)(((unsigned long long)(unsigned)t * p.page_mul) >> p.page_shift);
+            slot = t - column * p.page_size;
+            page = 0;
+            if (p.whole || ((there >> (lane & 15)) & 1)) page = __ldg(c.row + column);
         };
         // Read once per call: the stream must not push the code of the joins and the partial results out of L2 (1.3 GB:
         // 204 -> 200 us).
         const uint64_t policy = l2_policy_evict_first();
         const unsigned char *src;
-        uint32_t there;
         auto locate = [&](const Cursor &c) {
-            if (page == -1) atomicOr(p.status, DA_STATUS_BAD_PAGE_ID);   // the token is left out
-            there = __ballot_sync(DA_FULL_MASK, page >= 0);
+            const bool bad = (unsigned)page >= (unsigned)p.n_pages;
+            if (bad) {                             // the tokens are left out
+                atomicOr(p.status, DA_STATUS_BAD_PAGE_ID);
+                page = 0;
+            }
+            there &= ~__ballot_sync(DA_FULL_MASK, bad);
             src = p.pages + (c.head * p.page_head_stride + page * p.page_stride + slot * (2 * D)) * (long long)sizeof(T);
         };
         auto request = [&](int s) {
-            if (lane == 0) {
-                masks[warp][s] = there;
-                mbar_arrive_expect_tx(&bars[warp][s], (uint32_t)__popc(there) * TOKB);
+            unsigned char *dst = ring + s * STAGEB;
+            uint64_t *bar = &bars[warp][s];
+            if (p.whole && there == 0xffffu) {
+                if (elect_one()) {
+                    masks[warp][s] = 0xffffu;
+                    mbar_arrive_expect_tx(bar, kPagedUnit * TOKB);
+                    if constexpr (Math::kPitch == TOKB) {
+                        bulk_copy_g2s_hint(dst, src, kPagedUnit * TOKB, bar, policy);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < kPagedUnit; ++t) bulk_copy_g2s_hint(dst + t * Math::kPitch, src + t * TOKB, TOKB, bar, policy);
+                    }
+                }
+                __syncwarp();
+            } else {
+                if (lane == 0) {
+                    masks[warp][s] = there;
+                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * TOKB);
+                }
+                __syncwarp();
+                if (p.whole) src += lane * TOKB;
+                if (lane < kPagedUnit && ((there >> lane) & 1)) bulk_copy_g2s_hint(dst + lane * Math::kPitch, src, TOKB, bar, policy);
             }
-            __syncwarp();
-            if (page >= 0) bulk_copy_g2s_hint(ring + s * STAGEB + lane * Math::kPitch, src, TOKB, &bars[warp][s], policy);
         };
 
         int issued = 0;
@@ -444,7 +470,7 @@ static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
     return launch_dependent(kernel, dim3(kPagedCtas), dim3(WARPS * 32), (size_t)SMEM, stream, p);
 }
 
-constexpr int kPagedMaxWarps = 8;
+constexpr int kPagedMaxWarps = 12;
 // query rows that share a pass over the keys and values, float32: what the registers of a warp hold
 constexpr int paged_f32_rows(int head_dim) { return head_dim <= 64 ? 8 : (head_dim <= 128 ? 4 : 2); }
 constexpr int kPagedMmaRows = 16;

@@ -233,14 +233,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<uint32_t *>(&v);
 }
 
-// True in one lane of a converged warp.  Measured against a comparison of the lane number in front of the tensor-core and
-// copy instructions (16384 tokens x 32 heads): 1850 us, with this and a warp number read from one lane 1765.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0;
-}
-
 template <bool BF16>
 __global__ void __launch_bounds__(kPfThreads, 2)
 prefill_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

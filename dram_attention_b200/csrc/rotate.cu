@@ -49,13 +49,25 @@ struct RotateParams {
     int32_t *status;
 };
 
-// cos and sin of a fraction of `turns` full turns
-__device__ __forceinline__ float2 cos_sin_turns(double turns) {
-    const double quarters = 4.0 * turns;
-    const double k = rint(quarters);
-    float s, c;
-    sincospif(0.5f * (float)(quarters - k), &s, &c);      // |argument| <= 1/4: nothing is lost in the conversion
-    const int quadrant = (int)((long long)k & 3);
+// cos and sin of x quarter turns, |x| < 2^51.  x is split in 64 bits into its nearest whole number, whose low bits fall out of the
+// sum with 1.5 * 2^52, and a rest of at most 1/2, which loses nothing when it is rounded to 32 bits; the rest goes through
+// the Taylor series of sin and cos at (pi / 2) x, whose first left-out terms are below 2e-9 and 2e-10 there.
+__device__ __forceinline__ float2 cos_sin_quarters(double x) {
+    constexpr double kWhole = 6755399441055744.0, H = 1.5707963267948966;   // 1.5 * 2^52, pi / 2
+    constexpr double H2 = H * H, H3 = H2 * H, H4 = H2 * H2, H5 = H4 * H, H6 = H4 * H2, H7 = H6 * H, H8 = H4 * H4, H9 = H8 * H, H10 = H8 * H2;
+    const double shifted = x + kWhole;
+    const int quadrant = __double2loint(shifted) & 3;
+    const float f = (float)(x - (shifted - kWhole)), z = f * f;
+    float s = fmaf(z, (float)(H9 / 362880), -(float)(H7 / 5040));
+    s = fmaf(z, s, (float)(H5 / 120));
+    s = fmaf(z, s, -(float)(H3 / 6));
+    s = fmaf(z, s, (float)(H - (double)(float)H));          // (what pi / 2 loses in 32 bits)
+    s = fmaf(f, (float)H, f * s);
+    float c = fmaf(z, -(float)(H10 / 3628800), (float)(H8 / 40320));
+    c = fmaf(z, c, -(float)(H6 / 720));
+    c = fmaf(z, c, (float)(H4 / 24));
+    c = fmaf(z, c, -(float)(H2 / 2));
+    c = fmaf(z, c, 1.f);
     const float a = (quadrant & 1) ? s : c, b = (quadrant & 1) ? c : s;
     return make_float2((quadrant == 1 || quadrant == 2) ? -a : a, quadrant >= 2 ? -b : b);
 }
@@ -73,6 +85,12 @@ template <typename T, int V> struct Chunk {
     __device__ __forceinline__ void load(const T *p) { raw = __ldcs(reinterpret_cast<const Raw *>(p)); }
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<Raw *>(p) = raw; }
     __device__ __forceinline__ void zero() { raw = Raw{}; }
+    template <class At> __device__ __forceinline__ void gather(const T *p, At at) {
+        union { Raw r; T t[V]; } u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) u.t[i] = p[at(i)];
+        raw = u.r;
+    }
     __device__ __forceinline__ void unpack(float (&x)[V]) const {
         union { Raw r; T t[V]; uint32_t w[V > 1 ? V * sizeof(T) / 4 : 1]; } u;
         u.r = raw;
@@ -147,16 +165,22 @@ __device__ __forceinline__ Place find_place(const RotateParams &p, int row) {
     return at;
 }
 
-// HALF: channel i is paired with channel i + rot / 2; otherwise with its neighbour.  A thread's column: in front those that
-// rotate (both members' chunks of V channels; neighbours: one chunk that holds whole pairs, or the two channels of a pair when
-// V is 1), then those that copy a chunk behind the rotated part.
-template <typename T, int V, bool HALF, bool PAGED>
-__global__ void __launch_bounds__(512)
+// Which channels a thread has: in front the columns that rotate, then those that copy a chunk behind the rotated part.
+//   kNeighbours   channel 2 i is paired with 2 i + 1: one chunk of V channels, whole pairs (V 1: the two channels of a pair)
+//   kHalves       channel i is paired with i + rot / 2, a multiple of V: the chunks of both members
+//   kCrossed      the same where rot / 2 is no multiple of V: one chunk, the other members of its pairs read one by one
+//                 (2000 tokens of 16 + 4 heads, 17 pairs: channel by channel 44 us instead of 12)
+enum Pairing { kNeighbours, kHalves, kCrossed };
+
+// (three blocks of 384 threads on an SM: with a few registers more it is two, and a 32K append takes 147 us instead of 126)
+template <typename T, int V, Pairing PAIRING, bool PAGED>
+__global__ void __launch_bounds__(V > 1 ? 384 : 512, V > 1 ? (PAIRING == kNeighbours ? 3 : 2) : 1)
 rotate_kernel(const RotateParams p) {
-    constexpr bool kTwo = HALF || V == 1;         // a rotating column has two chunks
-    constexpr int kPairs = kTwo ? V : V / 2;      // its pairs
+    constexpr bool HALF = PAIRING == kHalves, CROSSED = PAIRING == kCrossed;
+    constexpr bool kTwo = HALF || (V == 1 && !CROSSED);          // a rotating column has two chunks
+    constexpr int kPairs = kTwo || CROSSED ? V : V / 2;          // pairs it takes part in
     extern __shared__ float2 cos_sin[];           // [tokens of the block][rot_half]
-    __shared__ long long sh_position[kRotateTokens];
+    __shared__ double sh_position[kRotateTokens];
     __shared__ long long sh_place[PAGED ? kRotateTokens : 1];   // offset in the pool, -1: no page, -2: a row of no sequence
     griddep_wait();
     griddep_launch_dependents();
@@ -183,6 +207,9 @@ rotate_kernel(const RotateParams p) {
 
     const T *base = static_cast<const T *>(p.src[kind]) + head0 * p.src_head[kind];
     const long long src_head = p.src_head[kind];
+    // crossed columns: where the partner of channel j stands, and which pair they are
+    auto partner = [&](int j) { const int c = at0 + j; return c < p.rot_half ? c + p.rot_half : (c < 2 * p.rot_half ? c - p.rot_half : c); };
+    auto pair_of = [&](int j) { const int c = at0 + j; return c < p.rot_half ? c : c - p.rot_half; };
     Chunk<T, V> a[kRotateRows], b[kRotateRows];
     auto request = [&](int t) {
         if (t >= here) return;
@@ -194,6 +221,9 @@ rotate_kernel(const RotateParams p) {
             if (i < mine) {
                 a[i].load(s + at0);
                 if (two) b[i].load(s + at1);
+                if constexpr (CROSSED) {
+                    if (turns) b[i].gather(s, partner);
+                }
             }
             s += src_head;
         }
@@ -206,39 +236,46 @@ rotate_kernel(const RotateParams p) {
         if constexpr (PAGED) {
             const Place at = find_place(p, t);
             if (at.status && blockIdx.y == 0) atomicOr(p.status, at.status);
-            sh_position[linear] = at.position;
+            sh_position[linear] = (double)at.position;
             sh_place[linear] = !at.used ? -2 : (at.page < 0 ? -1 : at.page * p.page_stride + (long long)at.slot * 2 * p.head_dim);
         } else {
             const int n = t / p.position_tokens;
             const long long i = n * p.position_batch + (t - n * p.position_tokens) * p.position_token;
-            sh_position[linear] = p.positions_64 ? __ldg(static_cast<const long long *>(p.positions) + i)
-                                                 : (long long)__ldg(static_cast<const int32_t *>(p.positions) + i);
+            sh_position[linear] = p.positions_64 ? (double)__ldg(static_cast<const long long *>(p.positions) + i)
+                                                 : (double)__ldg(static_cast<const int32_t *>(p.positions) + i);
         }
     }
     __syncthreads();
     for (int i = linear; i < here * p.rot_half; i += threads) {
         const int t = i / p.rot_half, pair = i - t * p.rot_half;
-        const double per_turn = (double)__ldg(p.inv_freq + pair) * 0.15915494309189535;   // 1 / 2 pi
-        const float2 cs = cos_sin_turns((double)sh_position[t] * per_turn);
+        const double quarters = (double)__ldg(p.inv_freq + pair) * 0.6366197723675814;   // 2 / pi
+        const float2 cs = cos_sin_quarters(sh_position[t] * quarters);
         cos_sin[i] = make_float2(cs.x * p.factor, cs.y * p.factor * p.sign);
     }
     __syncthreads();
 
     // a chunk that ends behind the rotated part: its last pairs are copied, not multiplied by 1 and 0
-    const int pairs = kTwo ? V : min(V / 2, p.rot_half - column * (V / 2));
+    const int pairs = CROSSED ? 2 * p.rot_half - at0 : (kTwo ? V : min(V / 2, p.rot_half - column * (V / 2)));
     const bool rotates = turns && kind != 2;
     const bool to_pages = PAGED && kind != 0;
     T *const out = to_pages ? static_cast<T *>(p.pages) + head0 * p.page_head_stride + (kind == 2 ? p.head_dim : 0)
                             : static_cast<T *>(p.dst[kind < 2 ? kind : 0]) + ((long long)first * p.heads[kind] + head0) * p.head_dim;
     const long long out_head = to_pages ? p.page_head_stride : p.head_dim;
     for (int t = z; t < here; t += blockDim.z) {
-        const float2 *cs = cos_sin + t * p.rot_half + column * kPairs;
+        const float2 *cs = cos_sin + t * p.rot_half + (CROSSED ? 0 : column * kPairs);
         const long long place = PAGED ? sh_place[t] : 0;
         T *d = out + (to_pages ? place : (long long)t * p.heads[kind] * p.head_dim);
         if (rotates) {
             float2 w[kPairs];
 #pragma unroll
-            for (int j = 0; j < kPairs; ++j) w[j] = kTwo || j < pairs ? cs[j] : make_float2(1.f, 0.f);
+            for (int j = 0; j < kPairs; ++j) {
+                if constexpr (CROSSED) {
+                    w[j] = j < pairs ? cs[pair_of(j)] : make_float2(1.f, 0.f);
+                    if (at0 + j < p.rot_half) w[j].y = -w[j].y;      // the first member of its pair
+                } else {
+                    w[j] = kTwo || j < pairs ? cs[j] : make_float2(1.f, 0.f);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kRotateRows; ++i) {
                 if (i >= mine) continue;
@@ -250,6 +287,12 @@ rotate_kernel(const RotateParams p) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) turn(x[j], u[j], w[j]);
                     b[i].pack(u);
+                } else if constexpr (CROSSED) {
+                    float u[V];
+                    b[i].unpack(u);
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (j < pairs) x[j] = x[j] * w[j].x + u[j] * w[j].y;
                 } else {
 #pragma unroll
                     for (int j = 0; j < V / 2; ++j)
@@ -276,10 +319,10 @@ rotate_kernel(const RotateParams p) {
     }
 }
 
-template <typename T, int V, bool HALF, bool PAGED>
+template <typename T, int V, Pairing PAIRING, bool PAGED>
 static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     const int rot = 2 * p.rot_half, d = p.head_dim;
-    const int columns = (HALF || V == 1) ? p.rot_half / V + (d - rot) / V : d / V;
+    const int columns = PAIRING == kHalves || (V == 1 && PAIRING == kNeighbours) ? p.rot_half / V + (d - rot) / V : d / V;
     p.all_tokens = n_batch * p.n_tokens;
     auto threads_for = [&](int each) {
         int y = 0;
@@ -300,7 +343,7 @@ static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     // halves: 105 us with blocks of 96 to 192 threads, 115 with 384; two tokens in turn 127), but for an append whose columns are one
     // chunk: the look-up of the places is then worth sharing (32 768 tokens: 126 us with 384 threads and two tokens in turn,
     // 136 with 128 and one).
-    constexpr bool kShare = PAGED && !HALF && V > 1;
+    constexpr bool kShare = PAGED && PAIRING == kNeighbours && V > 1;
     constexpr int THREADS = kShare ? 384 : 128;
     const int all_y = threads_for(p.rows_each);
     int y = columns * all_y <= 192 ? all_y : THREADS / columns;   // (the angles of a token are made once, then)
@@ -314,17 +357,24 @@ static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     const int rounds = kShare && p.all_tokens / z >= 2 * 8 * 148 ? 2 : 1;
     p.rounds = rounds;
     const int per_block = z * rounds;
-    return (int)launch_dependent(rotate_kernel<T, V, HALF, PAGED>, dim3((unsigned)(((long long)p.all_tokens + per_block - 1) / per_block), blocks_y),
+    return (int)launch_dependent(rotate_kernel<T, V, PAIRING, PAGED>, dim3((unsigned)(((long long)p.all_tokens + per_block - 1) / per_block), blocks_y),
                                  dim3(columns, y, z), (size_t)per_block * p.rot_half * sizeof(float2), stream, p);
 }
 
-// V: the longest access that every row and (halves) the second half start on a multiple of, up to 16 bytes
+// V: the longest access that every row starts on a multiple of, up to 16 bytes
+template <typename T, int V, bool PAGED>
+static int rotate_rows(const RotateParams &p, int n_batch, bool half, cudaStream_t stream) {
+    if (!half) return launch_rotate<T, V, kNeighbours, PAGED>(p, n_batch, stream);
+    if (p.rot_half % V == 0) return launch_rotate<T, V, kHalves, PAGED>(p, n_batch, stream);
+    if constexpr (V > 1) return launch_rotate<T, V, kCrossed, PAGED>(p, n_batch, stream);
+    return DA_ERR_UNSUPPORTED;   // (every size is a multiple of 1)
+}
 template <typename T, bool PAGED>
 static int rotate_by(const RotateParams &p, int n_batch, bool half, int v, cudaStream_t stream) {
     constexpr int MOST = 16 / (int)sizeof(T);
-    if (v >= MOST) return half ? launch_rotate<T, MOST, true, PAGED>(p, n_batch, stream) : launch_rotate<T, MOST, false, PAGED>(p, n_batch, stream);
-    if (v >= 2) return half ? launch_rotate<T, 2, true, PAGED>(p, n_batch, stream) : launch_rotate<T, 2, false, PAGED>(p, n_batch, stream);
-    return half ? launch_rotate<T, 1, true, PAGED>(p, n_batch, stream) : launch_rotate<T, 1, false, PAGED>(p, n_batch, stream);
+    if (v >= MOST) return rotate_rows<T, MOST, PAGED>(p, n_batch, half, stream);
+    if (v >= 2) return rotate_rows<T, 2, PAGED>(p, n_batch, half, stream);
+    return rotate_rows<T, 1, PAGED>(p, n_batch, half, stream);
 }
 
 template <bool PAGED>
@@ -387,7 +437,7 @@ extern "C" int da_rotate(const da_rotate_args *args) {
     p.positions = a.positions, p.positions_64 = a.positions_64 != 0;
     p.position_batch = a.position_strides[0], p.position_token = a.position_strides[1];
     const bool half = a.interleaved == 0;
-    const int v = access_elements(bases, strides | a.head_dim | (half ? p.rot_half : 0), esize);
+    const int v = access_elements(bases, strides | a.head_dim, esize);
     return rotate<false>(p, n_batch, (int)a.dtype, half, v, static_cast<cudaStream_t>(a.stream));
 }
 
@@ -433,6 +483,6 @@ extern "C" int da_append_pages(const da_append_pages_args *args) {
     p.lengths = a.lengths, p.starts = a.starts, p.n_sequences = (int)a.n_sequences;
     p.status = a.status;
     const bool half = a.interleaved == 0;
-    const int v = access_elements(bases, strides | a.head_dim | (half ? p.rot_half : 0), esize);
+    const int v = access_elements(bases, strides | a.head_dim, esize);
     return rotate<true>(p, 1, (int)a.dtype, half, v, static_cast<cudaStream_t>(a.stream));
 }
