@@ -16,10 +16,10 @@
 // tokens, 64 channels: 76 us, elected 64).  16-byte asynchronous copies of all lanes need fewer instructions still but
 // bring in less (64 sequences of 5000 tokens, 128 channels: 221 us against 197).
 //
-// An item that lies in one warp's stretch is written by the warp.  One that crosses warps is put together by the CTA from the
-// warps' partial results (row maximum, weight sum, accumulator: float32), and one that crosses CTAs by a second,
-// dependent launch from the CTAs' partial results: a CTA leaves at most two, for the item it begins in and the one it ends
-// in.  The joins go in the order of the line, so the same lengths give the same bits.
+// An item that lies in one warp's stretch is written by the warp.  Of one that does not, every warp leaves its partial result (row
+// maximum, weight sum, accumulator: float32) in the workspace, and a second, dependent launch joins them, in the order of
+// the line: the same lengths give the same bits.  (Joining the warps of a CTA in shared memory first leaves the second launch an
+// eighth of the rows, but its code, fetched when the stream has just ended, took 3 to 6 us.)
 #pragma once
 
 #include "da_common.cuh"
@@ -28,7 +28,7 @@ namespace da {
 
 constexpr int kPagedUnit = 16;        // tokens
 constexpr int kPagedCtas = 148;       // one per SM
-constexpr int kPagedMinUnits = 8;     // fewer are not worth a CTA of their own: a unit for every warp
+constexpr int kPagedMinUnits = 12;    // a CTA has at least these, if there is more than one: a unit for every warp
 
 struct PagedParams {
     const unsigned char *q;
@@ -46,8 +46,8 @@ struct PagedParams {
     int n_sequences, window;
     unsigned char *out;
     float *lse;
-    float *warp_partials;             // [CTA][warp][group_rows][D + 4]
-    float *cta_partials;              // [CTA][2][group_rows][D + 4]
+    float *partials;                  // [CTA][warp][2][group_rows][D + 4]: of the item that had begun before the warp's stretch,
+                                      // and of the one that begins in it and does not end there
     int32_t *status;
     int n_kv_heads, rep, groups, group_rows;   // query rows of a KV head, in groups of at most group_rows
     float scale_log2;
@@ -68,8 +68,8 @@ __device__ __forceinline__ Span span_of(const PagedParams &p, int length) {
 }
 
 // (a 64-bit division takes some hundred instructions; nearly every line is shorter than 2^32 units)
-__device__ __forceinline__ long long divide(long long n, int d) {
-    if ((n >> 32) == 0) return (long long)((uint32_t)n / (uint32_t)d);
+__device__ __forceinline__ long long divide(long long n, long long d) {
+    if (((n | d) >> 32) == 0) return (long long)((uint32_t)n / (uint32_t)d);
     return n / d;
 }
 
@@ -104,21 +104,29 @@ __device__ __forceinline__ Totals total_units(const PagedParams &p, int before, 
     return {all, front};
 }
 
-// How the line is dealt out: to as many CTAs as get kPagedMinUnits each, up to kPagedCtas, the first `more` of them one unit more.
+// How the line is dealt out: to as many CTAs as have kPagedMinUnits each, up to kPagedCtas, the first `more` of them one unit
+// more; inside a CTA to its warps in the same way.
 struct Deal {
     int ctas, more;
     long long each;
     __device__ __forceinline__ explicit Deal(long long total) {
-        const long long want = (total + kPagedMinUnits - 1) / kPagedMinUnits;
-        ctas = (int)(want < kPagedCtas ? want : kPagedCtas);
+        const long long most = total / kPagedMinUnits;
+        ctas = total <= 0 ? 0 : (most < 1 ? 1 : (most < kPagedCtas ? (int)most : kPagedCtas));
         each = ctas ? divide(total, ctas) : 0;
         more = (int)(total - each * ctas);
     }
     __device__ __forceinline__ long long begin(int c) const { return each * c + min(c, more); }
+    __device__ __forceinline__ int count(int c) const { return (int)each + (c < more); }
     __device__ __forceinline__ int cta_of(long long unit) const {
         const long long long_part = (each + 1) * more;
-        if (unit < long_part) return (int)(unit / (each + 1));
-        return more + (int)((unit - long_part) / each);
+        if (unit < long_part) return (int)divide(unit, each + 1);
+        return more + (int)divide(unit - long_part, each);
+    }
+    // warp of the CTA's unit `at` among `warps`
+    static __device__ __forceinline__ int warp_of(int count, int at, int warps) {
+        const int e = count / warps, m = count - e * warps;
+        if (at < (e + 1) * m) return at / (e + 1);
+        return m + (at - (e + 1) * m) / e;
     }
 };
 
@@ -227,227 +235,158 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     constexpr int D = Math::kD, PW = PagedRow<D>::kWidth;
     constexpr int ROWB = D * (int)sizeof(T), TOKB = 2 * ROWB;
     constexpr int STAGEB = kPagedUnit * Math::kPitch;
-    static_assert(STAGES * STAGEB >= Math::kRows * PW * 4, "a warp's ring holds its last partial result");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t bars[WARPS][STAGES];
     __shared__ uint32_t masks[WARPS][STAGES];      // tokens of the unit that are there
-    // What the warps leave to the CTA, in the order of the line: warp w its item that ended inside its stretch, if it had begun
-    // before (2 w, in global memory: the ring is busy), and its last one (2 w + 1, in its ring).
-    __shared__ int part_item[2 * WARPS];           // -1: none
-    __shared__ int part_flags[2 * WARPS];          // 1: the item begins in the warp's stretch, 2: it ends there
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
     if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) mbar_init(&bars[warp][s], 1);
-        part_item[2 * warp] = part_item[2 * warp + 1] = -1;
     }
     mbar_fence_init();
     __syncwarp();
     griddep_wait();
     griddep_launch_dependents();
 
-    // ---- this warp's stretch ------------------------------------------------------------
+    // this warp's stretch
     uint32_t first;
     const uint32_t first_sum = scan_units(p, 0, lane, first);
     const long long total = p.n_sequences <= 32 ? (long long)__shfl_sync(DA_FULL_MASK, first_sum, 31) : total_units(p, 0, lane).all;
     const Deal deal(total * (p.n_kv_heads * p.groups));
     if ((int)blockIdx.x >= deal.ctas) return;
     const long long lo = deal.begin(blockIdx.x);
-    const int mine = (int)deal.each + ((int)blockIdx.x < deal.more), spare = mine % WARPS;
+    const int mine = deal.count(blockIdx.x), spare = mine % WARPS;
     const int skip = mine / WARPS * warp + min(warp, spare);
     const int count = mine / WARPS + (warp < spare);
+    if (count == 0) return;
     unsigned char *ring = smem + (size_t)warp * STAGES * STAGEB;
 
-    if (count > 0) {
-        Cursor ahead;
-        ahead.seek(p, lo + skip, lane, first, first_sum);
-        Cursor at = ahead;
-        bool begins = at.u == at.s.u0;
+    Cursor ahead;
+    ahead.seek(p, lo + skip, lane, first, first_sum);
+    Cursor at = ahead;
+    bool begins = at.u == at.s.u0;
 
-        // The unit to be requested next: its tokens that there are, and its page (pages not whole: each lane's token's), looked
-        // up one unit ahead; then where it lies.
-        int page, slot;
-        uint32_t there;
-        auto look_up = [&](const Cursor &c) {
-            const int t0 = c.u * kPagedUnit, t = p.whole ? t0 : t0 + (lane & 15);
-            const int from = max(c.s.first - t0, 0), to = min(c.s.n - t0, kPagedUnit);
-            there = (0xffffu >> (kPagedUnit - to)) & (0xffffu << from);
-            const int column = (int)(((unsigned long long)(unsigned)t * p.page_mul) >> p.page_shift);
-            slot = t - column * p.page_size;
+    // The unit to be requested next: its tokens that there are, and its page (pages not whole: each lane's token's), looked
+    // up one unit ahead; then where it lies.
+    int page, slot;
+    uint32_t there;
+    auto look_up = [&](const Cursor &c) {
+        const int t0 = c.u * kPagedUnit, t = p.whole ? t0 : t0 + (lane & 15);
+        const int from = max(c.s.first - t0, 0), to = min(c.s.n - t0, kPagedUnit);
+        there = (0xffffu >> (kPagedUnit - to)) & (0xffffu << from);
+        const int column = (int)(((unsigned long long)(unsigned)t * p.page_mul) >> p.page_shift);
+        slot = t - column * p.page_size;
+        page = 0;
+        if (p.whole || ((there >> (lane & 15)) & 1)) page = __ldg(c.row + column);
+    };
+    // Read once per call: the stream must not push the code of the joins and the partial results out of L2 (1.3 GB:
+    // 204 -> 200 us).
+    const uint64_t policy = l2_policy_evict_first();
+    const unsigned char *src;
+    auto locate = [&](const Cursor &c) {
+        const bool bad = (unsigned)page >= (unsigned)p.n_pages;
+        if (bad) {                             // the tokens are left out
+            atomicOr(p.status, DA_STATUS_BAD_PAGE_ID);
             page = 0;
-            if (p.whole || ((there >> (lane & 15)) & 1)) page = __ldg(c.row + column);
-        };
-        // Read once per call: the stream must not push the code of the joins and the partial results out of L2 (1.3 GB:
-        // 204 -> 200 us).
-        const uint64_t policy = l2_policy_evict_first();
-        const unsigned char *src;
-        auto locate = [&](const Cursor &c) {
-            const bool bad = (unsigned)page >= (unsigned)p.n_pages;
-            if (bad) {                             // the tokens are left out
-                atomicOr(p.status, DA_STATUS_BAD_PAGE_ID);
-                page = 0;
-            }
-            there &= ~__ballot_sync(DA_FULL_MASK, bad);
-            src = p.pages + (c.head * p.page_head_stride + page * p.page_stride + slot * (2 * D)) * (long long)sizeof(T);
-        };
-        auto request = [&](int s) {
-            unsigned char *dst = ring + s * STAGEB;
-            uint64_t *bar = &bars[warp][s];
-            if (p.whole && there == 0xffffu) {
-                if (elect_one()) {
-                    masks[warp][s] = 0xffffu;
-                    mbar_arrive_expect_tx(bar, kPagedUnit * TOKB);
-                    if constexpr (Math::kPitch == TOKB) {
-                        bulk_copy_g2s_hint(dst, src, kPagedUnit * TOKB, bar, policy);
-                    } else {
+        }
+        there &= ~__ballot_sync(DA_FULL_MASK, bad);
+        src = p.pages + (c.head * p.page_head_stride + page * p.page_stride + slot * (2 * D)) * (long long)sizeof(T);
+    };
+    auto request = [&](int s) {
+        unsigned char *dst = ring + s * STAGEB;
+        uint64_t *bar = &bars[warp][s];
+        if (p.whole && there == 0xffffu) {
+            if (elect_one()) {
+                masks[warp][s] = 0xffffu;
+                mbar_arrive_expect_tx(bar, kPagedUnit * TOKB);
+                if constexpr (Math::kPitch == TOKB) {
+                    bulk_copy_g2s_hint(dst, src, kPagedUnit * TOKB, bar, policy);
+                } else {
 #pragma unroll
-                        for (int t = 0; t < kPagedUnit; ++t) bulk_copy_g2s_hint(dst + t * Math::kPitch, src + t * TOKB, TOKB, bar, policy);
-                    }
+                    for (int t = 0; t < kPagedUnit; ++t) bulk_copy_g2s_hint(dst + t * Math::kPitch, src + t * TOKB, TOKB, bar, policy);
                 }
-                __syncwarp();
-            } else {
-                if (lane == 0) {
-                    masks[warp][s] = there;
-                    mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * TOKB);
-                }
-                __syncwarp();
-                if (p.whole) src += lane * TOKB;
-                if (lane < kPagedUnit && ((there >> lane) & 1)) bulk_copy_g2s_hint(dst + lane * Math::kPitch, src, TOKB, bar, policy);
             }
-        };
+            __syncwarp();
+        } else {
+            if (lane == 0) {
+                masks[warp][s] = there;
+                mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * TOKB);
+            }
+            __syncwarp();
+            if (p.whole) src += lane * TOKB;
+            if (lane < kPagedUnit && ((there >> lane) & 1)) bulk_copy_g2s_hint(dst + lane * Math::kPitch, src, TOKB, bar, policy);
+        }
+    };
 
-        int issued = 0;
-        look_up(ahead);
-        for (; issued < STAGES && issued < count; ++issued) {
-            locate(ahead);
-            request(issued);
-            if (issued + 1 < count) {
+    int issued = 0;
+    look_up(ahead);
+    for (; issued < STAGES && issued < count; ++issued) {
+        locate(ahead);
+        request(issued);
+        if (issued + 1 < count) {
+            ahead.next(p);
+            look_up(ahead);
+        }
+    }
+
+    typename Math::State st;
+    int id = at.id(p);
+    int rows = rows_of(p, id);
+    Math::begin(st, p, at.b, at.head, at.group, rows, lane);
+    int s = 0;
+    uint32_t parity = 0;
+    for (int i = 0; i < count; ++i) {
+        if (issued < count) locate(ahead);
+        const bool arrived = mbar_wait_bounded(&bars[warp][s], parity);
+        if (!__all_sync(DA_FULL_MASK, arrived)) {
+            if (lane == 0) atomicOr(p.status, DA_STATUS_WAIT_TIMEOUT);
+            // the copies under way end before the shared memory is given up, or the wait for them does
+            for (; i < issued; ++i) {
+                mbar_wait_bounded(&bars[warp][s], parity);
+                if (++s == STAGES) s = 0, parity ^= 1;
+            }
+            break;
+        }
+        unsigned char *unit = ring + s * STAGEB;
+        const uint32_t mask = masks[warp][s];
+        if (mask != 0xffffu) {
+            // value rows that no token filled hold stale bytes: a weight of zero times one of them must be zero
+            for (int k = lane; k < kPagedUnit * (ROWB / 16); k += 32) {
+                const int t = k / (ROWB / 16);
+                if (!((mask >> t) & 1))
+                    *reinterpret_cast<uint4 *>(unit + t * Math::kPitch + ROWB + (k % (ROWB / 16)) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stage's next copies come after
+            __syncwarp();
+        }
+        Math::consume(st, unit, mask, lane, p.scale_log2);
+        __syncwarp();
+        if (issued < count) {
+            request(s);
+            if (++issued < count) {
                 ahead.next(p);
                 look_up(ahead);
             }
         }
-
-        typename Math::State st;
-        int id = at.id(p);
-        int rows = rows_of(p, id);
-        Math::begin(st, p, at.b, at.head, at.group, rows, lane);
-        int s = 0;
-        uint32_t parity = 0;
-        for (int i = 0; i < count; ++i) {
-            if (issued < count) locate(ahead);
-            const bool arrived = mbar_wait_bounded(&bars[warp][s], parity);
-            if (!__all_sync(DA_FULL_MASK, arrived)) {
-                if (lane == 0) atomicOr(p.status, DA_STATUS_WAIT_TIMEOUT);
-                // the copies under way end before the shared memory is given up, or the wait for them does
-                for (; i < issued; ++i) {
-                    mbar_wait_bounded(&bars[warp][s], parity);
-                    if (++s == STAGES) s = 0, parity ^= 1;
-                }
-                break;
-            }
-            unsigned char *unit = ring + s * STAGEB;
-            const uint32_t mask = masks[warp][s];
-            if (mask != 0xffffu) {
-                // value rows that no token filled hold stale bytes: a weight of zero times one of them must be zero
-                for (int k = lane; k < kPagedUnit * (ROWB / 16); k += 32) {
-                    const int t = k / (ROWB / 16);
-                    if (!((mask >> t) & 1))
-                        *reinterpret_cast<uint4 *>(unit + t * Math::kPitch + ROWB + (k % (ROWB / 16)) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stage's next copies come after
-                __syncwarp();
-            }
-            Math::consume(st, unit, mask, lane, p.scale_log2);
-            __syncwarp();
-            if (issued < count) {
-                request(s);
-                if (++issued < count) {
-                    ahead.next(p);
-                    look_up(ahead);
-                }
-            }
-            if (++s == STAGES) s = 0, parity ^= 1;
-            const bool ends = at.u + 1 == at.end;
-            if (!ends && i + 1 < count) {
-                ++at.u;
-                continue;
-            }
-            // ---- the item, or this warp's part of it, is done ------------------------------
-            if (begins && ends) {
-                Math::write(st, p, id, rows, lane);
-            } else {
-                const int k = 2 * warp + (i + 1 == count);
-                float *dst = i + 1 == count ? reinterpret_cast<float *>(ring)
-                                            : p.warp_partials + ((size_t)blockIdx.x * WARPS + warp) * p.group_rows * PW;
-                Math::publish(st, dst, lane, rows);
-                if (lane == 0) {
-                    part_item[k] = id;
-                    part_flags[k] = (begins ? 1 : 0) | (ends ? 2 : 0);
-                }
-            }
-            if (i + 1 < count) {
-                at.next(p);
-                id = at.id(p);
-                rows = rows_of(p, id);
-                begins = true;
-                Math::begin(st, p, at.b, at.head, at.group, rows, lane);
-            }
+        if (++s == STAGES) s = 0, parity ^= 1;
+        const bool ends = at.u + 1 == at.end;
+        if (!ends && i + 1 < count) {
+            ++at.u;
+            continue;
         }
-    }
-    __syncthreads();
-
-    // ---- items that cross warps: one task per item, row and four channels ------------------------------
-    constexpr int COLS = D / 4;
-    const int item_of = lane < 2 * WARPS ? part_item[lane] : -1;
-    const unsigned there = __ballot_sync(DA_FULL_MASK, item_of >= 0);
-    const unsigned in_front = there & ((1u << lane) - 1);
-    const int item_before = __shfl_sync(DA_FULL_MASK, item_of, in_front ? 31 - __clz(in_front) : 0);
-    unsigned leads = __ballot_sync(DA_FULL_MASK, item_of >= 0 && (!in_front || item_before != item_of));
-    const int n_items = __popc(leads);
-    const int tasks = p.group_rows * COLS;
-    int at_item = 0;                               // leads: from this item on
-    for (int t = threadIdx.x; t < n_items * tasks; t += WARPS * 32) {
-        const int g = t / tasks, e = t - g * tasks;
-        const int r = e / COLS, c = e - r * COLS;
-        for (; at_item < g; ++at_item) leads &= leads - 1;
-        const int begin = __ffs(leads) - 1;
-        const unsigned behind = leads & (leads - 1);
-        unsigned parts = there & ~((1u << begin) - 1);
-        if (behind) parts &= (behind & -behind) - 1;
-        const int id = part_item[begin];
-        if (r >= rows_of(p, id)) continue;
-        const bool begins = part_flags[begin] & 1, ends = part_flags[31 - __clz(parts)] & 2;
-        PartialSum x;
-        x.clear();
-        while (parts) {
-            constexpr int N = 4;
-            float2 ml[N];
-            float4 v[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                ml[i] = make_float2(-INFINITY, 0.f);
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (parts) {
-                    const int k = __ffs(parts) - 1;
-                    parts &= parts - 1;
-                    const float *row = (k & 1 ? reinterpret_cast<const float *>(smem + (size_t)(k >> 1) * STAGES * STAGEB)
-                                              : p.warp_partials + ((size_t)blockIdx.x * WARPS + (k >> 1)) * p.group_rows * PW) + r * PW;
-                    ml[i] = *reinterpret_cast<const float2 *>(row + D);
-                    v[i] = *reinterpret_cast<const float4 *>(row + 4 * c);
-                }
-            }
-            x.add(ml, v);
-        }
+        // the item, or this warp's part of it, is done
         if (begins && ends) {
-            size_t index;
-            T *out = out_row<T>(p, id, r, D, index);
-            store_divided(out + 4 * c, x.o, x.l);
-            if (c == 0 && p.lse) p.lse[index] = natural_lse(x.m, x.l);
+            Math::write(st, p, id, rows, lane);
         } else {
-            float *dst = p.cta_partials + (((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * p.group_rows + r) * PW;
-            *reinterpret_cast<float4 *>(dst + 4 * c) = x.o;
-            if (c == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(x.m, x.l);
+            Math::publish(st, p.partials + (((size_t)blockIdx.x * WARPS + warp) * 2 + (begins ? 1 : 0)) * p.group_rows * PW, lane, rows);
+        }
+        if (i + 1 < count) {
+            at.next(p);
+            id = at.id(p);
+            rows = rows_of(p, id);
+            begins = true;
+            Math::begin(st, p, at.b, at.head, at.group, rows, lane);
         }
     }
 }
@@ -470,10 +409,14 @@ static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
     return launch_dependent(kernel, dim3(kPagedCtas), dim3(WARPS * 32), (size_t)SMEM, stream, p);
 }
 
-constexpr int kPagedMaxWarps = 12;
 // query rows that share a pass over the keys and values, float32: what the registers of a warp hold
 constexpr int paged_f32_rows(int head_dim) { return head_dim <= 64 ? 8 : (head_dim <= 128 ? 4 : 2); }
 constexpr int kPagedMmaRows = 16;
+
+
+// Warps of the CTAs of paged_attention_kernel.
+__host__ __device__ constexpr int paged_mma_warps(int head_dim) { return head_dim > 128 ? 6 : head_dim > 96 ? 8 : 12; }
+__host__ __device__ constexpr int paged_f32_warps(int head_dim) { return head_dim > 128 ? 3 : head_dim > 96 ? 6 : 8; }
 
 cudaError_t paged_attention_f32(const PagedParams &p, int head_dim, cudaStream_t stream);
 cudaError_t paged_attention_f16(const PagedParams &p, int head_dim, cudaStream_t stream);

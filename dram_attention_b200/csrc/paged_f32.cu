@@ -168,8 +168,8 @@ struct PagedSimt {
 
 // As few rows as the group has: fewer instructions per unit, and less code, which a short call fetches from memory.
 // (warps x stages x 16 tokens of 8 D bytes: 160 to 197 KB; more than 8 warps would have 168 registers)
-template <int D, int WARPS, int STAGES> static cudaError_t paged_simt(const PagedParams &p, cudaStream_t stream) {
-    constexpr int MOST = paged_f32_rows(D);
+template <int D, int STAGES> static cudaError_t paged_simt(const PagedParams &p, cudaStream_t stream) {
+    constexpr int MOST = paged_f32_rows(D), WARPS = paged_f32_warps(D);
     if (p.group_rows <= 1) return launch_paged<PagedSimt<D, 1>, WARPS, STAGES>(p, stream);
     if constexpr (MOST > 2) {
         if (p.group_rows <= 2) return launch_paged<PagedSimt<D, 2>, WARPS, STAGES>(p, stream);
@@ -182,11 +182,11 @@ template <int D, int WARPS, int STAGES> static cudaError_t paged_simt(const Page
 
 cudaError_t paged_attention_f32(const PagedParams &p, int head_dim, cudaStream_t stream) {
     switch (head_dim) {
-    case 64: return paged_simt<64, 8, 3>(p, stream);
-    case 80: return paged_simt<80, 8, 2>(p, stream);
-    case 96: return paged_simt<96, 8, 2>(p, stream);
-    case 128: return paged_simt<128, 6, 2>(p, stream);
-    default: return paged_simt<256, 3, 2>(p, stream);
+    case 64: return paged_simt<64, 3>(p, stream);
+    case 80: return paged_simt<80, 2>(p, stream);
+    case 96: return paged_simt<96, 2>(p, stream);
+    case 128: return paged_simt<128, 2>(p, stream);
+    default: return paged_simt<256, 2>(p, stream);
     }
 }
 

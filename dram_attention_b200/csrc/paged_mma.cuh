@@ -151,16 +151,15 @@ struct PagedMma {
     }
 };
 
-// As many stages as fit for the number of warps that is fastest.  A stage stands empty from the arrival of its unit until the warp
-// is through with it: with 128 channels and twelve warps there are two stages each and half the ring is empty at times, and the
-// threads have 168 registers, too few; eight have three (64 sequences of 5000 tokens 234 -> 203 us, one of 131 072
-// 95 -> 87).  Smaller heads have units of fewer bytes, so more of them have to be worked on at a time: twelve (60
-// sequences of 3000 tokens with 64, 80, 96 channels: 64, 76, 89 us, with eight warps 80 to 100).  The accumulators of 256
-// channels leave registers for six (265 us; with four warps of three stages 289).
+// As many stages as fit for the number of warps that is fastest, but two for 128 channels: 135 KB under way on every SM are enough
+// (64 sequences of 5000 tokens, 1.3 GB: eight warps of three or two stages 206 us, seven of three 211, ten or twelve of two 211,
+// whose threads have too few registers).  Smaller heads have units of fewer bytes, so more of them have to be worked on at a
+// time: twelve (60 sequences of 3000 tokens with 64, 80, 96 channels: 64, 76, 89 us, with eight warps 80 to 100).  The
+// accumulators of 256 channels leave registers for six (265 us; with four warps of three stages 289).
 template <int D> struct PagedMmaShape {
     static constexpr int kStage = kPagedUnit * (4 * D + 16);
-    static constexpr int kWarps = D > 128 ? 6 : D > 96 ? 8 : 12;
-    static constexpr int kStages = (220 * 1024) / (kWarps * kStage);
+    static constexpr int kWarps = paged_mma_warps(D);
+    static constexpr int kStages = D == 128 ? 2 : (220 * 1024) / (kWarps * kStage);
     static_assert(kStages >= 2, "");
 };
 
