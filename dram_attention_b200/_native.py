@@ -83,7 +83,7 @@ _SIGNATURES = {
                                c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "da_rotate": (c_int, [c_char_p]),
     "da_append_pages": (c_int, [c_char_p]),
-    "da_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "da_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "da_paged_attention": (c_int, [c_char_p]),
 }
 

@@ -17,8 +17,8 @@
 // bring in less (64 sequences of 5000 tokens, 128 channels: 221 us against 197).
 //
 // An item that lies in one warp's stretch is written by the warp.  Of one that does not, every warp leaves its partial result (row
-// maximum, weight sum, accumulator: float32) in the workspace, and a second, dependent launch joins them, in the order of
-// the line: the same lengths give the same bits.  (Joining the warps of a CTA in shared memory first leaves the second launch an
+// maximum, weight sum, accumulator: float32) in the workspace; the warps an item begins and ends in note their numbers there; and a
+// second, dependent launch joins the parts, in the order of the line: the same lengths give the same bits.  (Joining the warps of a CTA in shared memory first leaves the second launch an
 // eighth of the rows, but its code, fetched when the stream has just ended, took 3 to 6 us.)
 #pragma once
 
@@ -48,6 +48,7 @@ struct PagedParams {
     float *lse;
     float *partials;                  // [CTA][warp][2][group_rows][D + 4]: of the item that had begun before the warp's stretch,
                                       // and of the one that begins in it and does not end there
+    int2 *spans;                      // [item]: the warps (numbered through all CTAs) it begins and ends in
     int32_t *status;
     int n_kv_heads, rep, groups, group_rows;   // query rows of a KV head, in groups of at most group_rows
     float scale_log2;
@@ -196,6 +197,7 @@ struct PartialSum {
     float m, l;
     float4 o;
     __device__ __forceinline__ void clear() { m = -INFINITY, l = 0.f, o = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void add_lane(int off);     // what the lane `off` across has
     template <int N> __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&v)[N]) {
         float mx = m;
 #pragma unroll
@@ -213,6 +215,13 @@ struct PartialSum {
         }
     }
 };
+
+__device__ __forceinline__ void PartialSum::add_lane(int off) {
+    const float2 ml[1] = {make_float2(__shfl_xor_sync(DA_FULL_MASK, m, off), __shfl_xor_sync(DA_FULL_MASK, l, off))};
+    const float4 v[1] = {make_float4(__shfl_xor_sync(DA_FULL_MASK, o.x, off), __shfl_xor_sync(DA_FULL_MASK, o.y, off),
+                                     __shfl_xor_sync(DA_FULL_MASK, o.z, off), __shfl_xor_sync(DA_FULL_MASK, o.w, off))};
+    add(ml, v);
+}
 
 // Four consecutive elements, divided by the weight sum.
 template <typename T> __device__ __forceinline__ void store_divided(T *dst, const float4 &o, float l) {
@@ -376,6 +385,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             continue;
         }
         // the item, or this warp's part of it, is done
+        if (lane == 0) {
+            if (begins) p.spans[id].x = blockIdx.x * WARPS + warp;
+            if (ends) p.spans[id].y = blockIdx.x * WARPS + warp;
+        }
         if (begins && ends) {
             Math::write(st, p, id, rows, lane);
         } else {

@@ -168,7 +168,7 @@ class PagedKVCache:
         lse = torch.empty(n, hq, dtype=torch.float32, device=q.device) if return_lse else None
         if n:
             # scratch of this call alone: two captured steps, or two streams, never share it
-            size, like = self._scratch.get(rep) or self._scratch_like(rep)
+            size, like = self._scratch.get((n, rep)) or self._scratch_like(n, rep)
             scratch = torch.empty_like(like)
             _native.launch(_native.lib().da_paged_attention, _native.PACK_ATTEND(
                 q.data_ptr(), strides[0], strides[1], *self._pool, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
@@ -177,10 +177,13 @@ class PagedKVCache:
                 self.head_dim, self._dtype_code, _native.stream_of(self._device)), self._device, "da_paged_attention")
         return (out, lse) if return_lse else out
 
-    def _scratch_like(self, rep: int):
-        """Bytes of scratch for `rep` query heads per KV head, and a tensor of that many elements (one byte of memory) to make it like"""
-        size = _native.lib().da_paged_attention_workspace_bytes(rep, self.head_dim, self._dtype_code)
-        entry = self._scratch[rep] = (size, torch.empty(1, dtype=torch.uint8, device=self.pages.device).expand(max(size, 16)))
+    def _scratch_like(self, n: int, rep: int):
+        """Bytes of scratch for n sequences with `rep` query heads per KV head, and a tensor of that many elements (one byte of
+        memory) to make it like"""
+        size = _native.lib().da_paged_attention_workspace_bytes(n, self.n_kv_heads, rep, self.head_dim, self._dtype_code)
+        if len(self._scratch) >= 256:
+            self._scratch.clear()
+        entry = self._scratch[n, rep] = (size, torch.empty(1, dtype=torch.uint8, device=self.pages.device).expand(max(size, 16)))
         return entry
 
     def check_status(self) -> None:

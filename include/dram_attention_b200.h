@@ -725,7 +725,8 @@ typedef struct da_paged_attention_args {
     int64_t n_kv_heads, rep, head_dim, dtype;
     da_stream_t stream;
 } da_paged_attention_args;
-DA_API size_t da_paged_attention_workspace_bytes(int rep, int head_dim, int dtype);   /* 0: not a shape of the call */
+/* 0: not a shape of the call */
+DA_API size_t da_paged_attention_workspace_bytes(int n_sequences, int n_kv_heads, int rep, int head_dim, int dtype);
 DA_API int da_paged_attention(const da_paged_attention_args *args);
 
 #ifdef __cplusplus

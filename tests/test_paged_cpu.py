@@ -79,10 +79,10 @@ def test_attend_refuses(native, changes, code):
 
 @pytest.mark.parametrize("rep,d,dtype", [(1, 64, 2), (4, 128, 1), (16, 128, 2), (17, 256, 2), (5, 80, 0), (256, 96, 0)])
 def test_attend_workspace_has_to_be_as_large_as_stated(native, rep, d, dtype):
-    need = native.lib().da_paged_attention_workspace_bytes(rep, d, dtype)
-    assert need > 0
+    need = native.lib().da_paged_attention_workspace_bytes(2, 2, rep, d, dtype)
+    assert need > 0 and native.lib().da_paged_attention_workspace_bytes(200, 2, rep, d, dtype) > need
     assert _call(native, "da_paged_attention", ATTEND, ATTEND_OK, rep=rep, head_dim=d, dtype=dtype, workspace_bytes=need - 1) == WORKSPACE
-    for bad in ((0, 64, 2), (257, 64, 2), (4, 72, 2), (4, 64, 3), (-1, 64, 0)):
+    for bad in ((2, 2, 0, 64, 2), (2, 2, 257, 64, 2), (2, 2, 4, 72, 2), (2, 2, 4, 64, 3), (2, 2, -1, 64, 0), (0, 2, 4, 64, 0), (2, 0, 4, 64, 0)):
         assert native.lib().da_paged_attention_workspace_bytes(*bad) == 0
 
 
