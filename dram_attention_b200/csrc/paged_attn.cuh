@@ -236,7 +236,8 @@ template <typename T> __device__ __forceinline__ void store_divided(T *dst, cons
     }
 }
 
-// Math: the arithmetic of a unit.  kD, kPitch (bytes of a token in shared memory), State, begin (query rows),
+// Math: the arithmetic of a unit.  kD, kPitch (bytes of a token in shared memory), kScratch (bytes of a
+// warp's own), State, begin (query rows),
 // consume (one unit), publish (a partial result), write (a complete one).
 template <class Math, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const PagedParams p) {
@@ -270,6 +271,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     const int count = mine / WARPS + (warp < spare);
     if (count == 0) return;
     unsigned char *ring = smem + (size_t)warp * STAGES * STAGEB;
+    unsigned char *scratch = smem + (size_t)WARPS * STAGES * STAGEB + (size_t)warp * Math::kScratch;
 
     Cursor ahead;
     ahead.seek(p, lo + skip, lane, first, first_sum);
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     typename Math::State st;
     int id = at.id(p);
     int rows = rows_of(p, id);
-    Math::begin(st, p, at.b, at.head, at.group, rows, lane);
+    Math::begin(st, p, at.b, at.head, at.group, rows, lane, scratch);
     int s = 0;
     uint32_t parity = 0;
     for (int i = 0; i < count; ++i) {
@@ -399,14 +401,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             id = at.id(p);
             rows = rows_of(p, id);
             begins = true;
-            Math::begin(st, p, at.b, at.head, at.group, rows, lane);
+            Math::begin(st, p, at.b, at.head, at.group, rows, lane, scratch);
         }
     }
 }
 
 template <class Math, int WARPS, int STAGES>
 static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
-    constexpr int SMEM = WARPS * STAGES * kPagedUnit * Math::kPitch;
+    constexpr int SMEM = WARPS * (STAGES * kPagedUnit * Math::kPitch + Math::kScratch);
     static_assert(SMEM <= 224 * 1024, "");
     auto kernel = paged_attention_kernel<Math, WARPS, STAGES>;
     static bool ready[64] = {};
@@ -423,7 +425,7 @@ static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
 }
 
 // query rows that share a pass over the keys and values, float32: what the registers of a warp hold
-constexpr int paged_f32_rows(int head_dim) { return head_dim <= 64 ? 8 : (head_dim <= 128 ? 4 : 2); }
+constexpr int paged_f32_rows(int head_dim) { return head_dim <= 128 ? 8 : 4; }
 constexpr int kPagedMmaRows = 16;
 
 

@@ -20,6 +20,7 @@ struct PagedMma {
     static constexpr int kD = D_, kRows = FULL ? 16 : 8;
     static constexpr int ROWB = kD * 2, kPitch = 2 * ROWB + 16;
     static constexpr int KSTEPS = kD / 16, NT = kD / 8, NR = FULL ? 2 : 1;
+    static constexpr int kScratch = 0;
     static_assert(kD % 16 == 0, "whole k-steps");
 
     struct State {
@@ -28,7 +29,7 @@ struct PagedMma {
         float o[NT][4];
     };
 
-    __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int head, int group, int rows, int lane) {
+    __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int head, int group, int rows, int lane, unsigned char *) {
         const int head0 = head * p.rep + group * p.group_rows;
 #pragma unroll
         for (int half = 0; half < NR; ++half) {
