@@ -28,7 +28,6 @@ namespace da {
 
 constexpr int kPagedUnit = 16;        // tokens
 constexpr int kPagedCtas = 148;       // one per SM
-constexpr int kPagedMinUnits = 12;    // a CTA has at least these, if there is more than one: a unit for every warp
 
 struct PagedParams {
     const unsigned char *q;
@@ -105,13 +104,13 @@ __device__ __forceinline__ Totals total_units(const PagedParams &p, int before, 
     return {all, front};
 }
 
-// How the line is dealt out: to as many CTAs as have kPagedMinUnits each, up to kPagedCtas, the first `more` of them one unit
-// more; inside a CTA to its warps in the same way.
+// How the line is dealt out: to as many CTAs as have a unit for each of their `warps`, up to kPagedCtas, the first `more` of them
+// one unit more; inside a CTA to its warps in the same way.
 struct Deal {
     int ctas, more;
     long long each;
-    __device__ __forceinline__ explicit Deal(long long total) {
-        const long long most = total / kPagedMinUnits;
+    __device__ __forceinline__ Deal(long long total, int warps) {
+        const long long most = divide(total, warps);
         ctas = total <= 0 ? 0 : (most < 1 ? 1 : (most < kPagedCtas ? (int)most : kPagedCtas));
         each = ctas ? divide(total, ctas) : 0;
         more = (int)(total - each * ctas);
@@ -263,7 +262,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     uint32_t first;
     const uint32_t first_sum = scan_units(p, 0, lane, first);
     const long long total = p.n_sequences <= 32 ? (long long)__shfl_sync(DA_FULL_MASK, first_sum, 31) : total_units(p, 0, lane).all;
-    const Deal deal(total * (p.n_kv_heads * p.groups));
+    const Deal deal(total * (p.n_kv_heads * p.groups), WARPS);
     if ((int)blockIdx.x >= deal.ctas) return;
     const long long lo = deal.begin(blockIdx.x);
     const int mine = deal.count(blockIdx.x), spare = mine % WARPS;

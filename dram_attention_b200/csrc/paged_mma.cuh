@@ -72,7 +72,9 @@ struct PagedMma {
             mma(ks & 1 ? t0 : s0, a, b[0], b[1]);
             mma(ks & 1 ? t1 : s1, a, b[2], b[3]);
         }
-        uint32_t pa[NR][2];
+        // The weights take part in the second product as the sum of two 16-bit numbers: rounded to one, they alone put bfloat16
+        // outputs 1.2 times as far from the 64-bit ones as their own rounding does, and memory hides the products.
+        uint32_t pa[NR][2], pb[NR][2];
 #pragma unroll
         for (int half = 0; half < NR; ++half) {
             // this lane: row lane / 4 + 8 * half, tokens 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
@@ -103,6 +105,12 @@ struct PagedMma {
             }
             pa[half][0] = MmaTraits<T>::pack(v[0], v[1]);
             pa[half][1] = MmaTraits<T>::pack(v[2], v[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float lo, hi;
+                unpack2<T>(pa[half][i], lo, hi);
+                pb[half][i] = MmaTraits<T>::pack(v[2 * i] - lo, v[2 * i + 1] - hi);
+            }
         }
 #pragma unroll
         for (int d = 0; d < NT / 2; ++d) {
@@ -110,6 +118,8 @@ struct PagedMma {
             ldmatrix_x4_trans(b, values + d * 32);
             mma(st.o[2 * d], pa, b[0], b[1]);
             mma(st.o[2 * d + 1], pa, b[2], b[3]);
+            mma(st.o[2 * d], pb, b[0], b[1]);
+            mma(st.o[2 * d + 1], pb, b[2], b[3]);
         }
     }
 
