@@ -67,12 +67,12 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParam
     if constexpr (!MANY) {
         // (the lengths were complete before the launch that this one follows let it in)
         if (warp == 0) {
-            const Totals units = total_units(p, b, lane);
+            const Survey survey(p, lane);
             length = __ldg(p.lengths + b);
             const int mine = span_of(p, length).units;
             if (mine) {
-                const long long begin = units.before * per + (long long)(item % per) * mine;
-                const Deal deal(units.all * per, MAIN_WARPS);
+                const long long begin = survey.before(p, b, lane) * per + (long long)(item % per) * mine;
+                const Deal deal(survey.total() * per, MAIN_WARPS);
                 const int c0 = deal.cta_of(begin), c1 = deal.cta_of(begin + mine - 1);
                 span.x = c0 * MAIN_WARPS + Deal::warp_of(deal.count(c0), (int)(begin - deal.begin(c0)), MAIN_WARPS);
                 span.y = c1 * MAIN_WARPS + Deal::warp_of(deal.count(c1), (int)(begin + mine - 1 - deal.begin(c1)), MAIN_WARPS);

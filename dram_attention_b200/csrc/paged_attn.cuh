@@ -73,36 +73,56 @@ __device__ __forceinline__ long long divide(long long n, long long d) {
     return n / d;
 }
 
-// Units per (head, group) of 32 sequences from b0 on, one per lane, and their inclusive sums (below 2^32: 32 times 2^27).
-__device__ __forceinline__ uint32_t scan_units(const PagedParams &p, int b0, int lane, uint32_t &mine) {
-    mine = b0 + lane < p.n_sequences ? span_of(p, __ldg(p.lengths + b0 + lane)).units : 0;
-    uint32_t sum = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t v = __shfl_up_sync(DA_FULL_MASK, sum, off);
-        if (lane >= off) sum += v;
-    }
-    return sum;
+__device__ __forceinline__ long long shfl_64(long long v, int from) {
+    const int lo = __shfl_sync(DA_FULL_MASK, (int)(v & 0xffffffff), from);
+    const int hi = __shfl_sync(DA_FULL_MASK, (int)(v >> 32), from);
+    return ((long long)hi << 32) | (unsigned)lo;
 }
 
-// Units per (head, group) of all sequences, and of those in front of `before`.
-struct Totals {
-    long long all, before;
-};
-__device__ __forceinline__ Totals total_units(const PagedParams &p, int before, int lane) {
-    long long all = 0, front = 0;
-    for (int b = lane; b < p.n_sequences; b += 32) {
-        const int u = span_of(p, __ldg(p.lengths + b)).units;
-        all += u;
-        if (b < before) front += u;
-    }
+// Units per (head, group) of the sequences, a lane for a run of `each` consecutive ones, and their sums up to the lane's run.
+struct Survey {
+    int each;
+    long long mine, sum;
+    __device__ __forceinline__ Survey(const PagedParams &p, int lane) {
+        each = (p.n_sequences + 31) >> 5;
+        if (each == 1) {                           // (below 2^32: 32 times 2^27)
+            const uint32_t u = lane < p.n_sequences ? span_of(p, __ldg(p.lengths + lane)).units : 0;
+            uint32_t v = u;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        all += __shfl_xor_sync(DA_FULL_MASK, all, off);
-        front += __shfl_xor_sync(DA_FULL_MASK, front, off);
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t w = __shfl_up_sync(DA_FULL_MASK, v, off);
+                if (lane >= off) v += w;
+            }
+            mine = u, sum = v;
+            return;
+        }
+        mine = 0;
+        const int end = min((lane + 1) * each, p.n_sequences);
+#pragma unroll 4
+        for (int b = lane * each; b < end; ++b) mine += span_of(p, __ldg(p.lengths + b)).units;
+        sum = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int lo = __shfl_up_sync(DA_FULL_MASK, (int)(sum & 0xffffffff), off);
+            const int hi = __shfl_up_sync(DA_FULL_MASK, (int)(sum >> 32), off);
+            if (lane >= off) sum += ((long long)hi << 32) | (unsigned)lo;
+        }
     }
-    return {all, front};
-}
+    __device__ __forceinline__ long long total() const { return shfl_64(sum, 31); }
+    // of the sequences in front of `b`
+    __device__ __forceinline__ long long before(const PagedParams &p, int b, int lane) const {
+        const int l = b / each;
+        long long front = shfl_64(sum - mine, l);
+        if (each > 1) {
+            long long u = 0;
+            for (int i = l * each + lane; i < b; i += 32) u += span_of(p, __ldg(p.lengths + i)).units;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) u += __shfl_xor_sync(DA_FULL_MASK, u, off);
+            front += u;
+        }
+        return front;
+    }
+};
 
 // How the line is dealt out: to as many CTAs as have a unit for each of their `warps`, up to kPagedCtas, the first `more` of them
 // one unit more; inside a CTA to its warps in the same way.
@@ -158,20 +178,35 @@ struct Cursor {
         }
         u = s.u0;
     }
-    // to unit `at` of the line; mine, sum: scan_units of the first 32 sequences
-    __device__ __forceinline__ void seek(const PagedParams &p, long long at, int lane, uint32_t mine, uint32_t sum) {
+    // to unit `at` of the line
+    __device__ __forceinline__ void seek(const PagedParams &p, long long at, int lane, const Survey &survey) {
         const int per = p.n_kv_heads * p.groups;
-        long long front = 0;
-        int b0 = 0;
-        unsigned past;
-        while ((past = __ballot_sync(DA_FULL_MASK, (front + sum) * per > at)) == 0 && b0 + 32 < p.n_sequences) {
-            front += __shfl_sync(DA_FULL_MASK, sum, 31);
-            b0 += 32;
-            sum = scan_units(p, b0, lane, mine);
+        const unsigned past = __ballot_sync(DA_FULL_MASK, survey.sum * per > at);
+        const int l = past ? __ffs(past) - 1 : 31;
+        long long front = shfl_64(survey.sum - survey.mine, l);
+        int sequence = l * survey.each;
+        if (survey.each > 1) {
+            // inside the lane's run, 32 sequences at a time (their sums below 2^32)
+            for (int b0 = sequence;; b0 += 32) {
+                const int b = b0 + lane;
+                const uint32_t u = b < min(sequence + survey.each, p.n_sequences) ? span_of(p, __ldg(p.lengths + b)).units : 0;
+                uint32_t v = u;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const uint32_t w = __shfl_up_sync(DA_FULL_MASK, v, off);
+                    if (lane >= off) v += w;
+                }
+                const unsigned here = __ballot_sync(DA_FULL_MASK, (front + v) * per > at);
+                if (here || b0 + 32 >= sequence + survey.each) {
+                    const int i = here ? __ffs(here) - 1 : 0;
+                    front += __shfl_sync(DA_FULL_MASK, v - u, i);
+                    sequence = b0 + i;
+                    break;
+                }
+                front += __shfl_sync(DA_FULL_MASK, v, 31);
+            }
         }
-        const int l = past ? __ffs(past) - 1 : 0;
-        front += __shfl_sync(DA_FULL_MASK, sum - mine, l);
-        enter(p, min(b0 + l, p.n_sequences - 1));
+        enter(p, min(sequence, p.n_sequences - 1));
         const long long inside = at - front * per;
         const int item = (int)divide(inside, max(s.units, 1));
         head = item / p.groups;
@@ -259,10 +294,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     griddep_launch_dependents();
 
     // this warp's stretch
-    uint32_t first;
-    const uint32_t first_sum = scan_units(p, 0, lane, first);
-    const long long total = p.n_sequences <= 32 ? (long long)__shfl_sync(DA_FULL_MASK, first_sum, 31) : total_units(p, 0, lane).all;
-    const Deal deal(total * (p.n_kv_heads * p.groups), WARPS);
+    const Survey survey(p, lane);
+    const Deal deal(survey.total() * (p.n_kv_heads * p.groups), WARPS);
     if ((int)blockIdx.x >= deal.ctas) return;
     const long long lo = deal.begin(blockIdx.x);
     const int mine = deal.count(blockIdx.x), spare = mine % WARPS;
@@ -273,7 +306,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     unsigned char *scratch = smem + (size_t)WARPS * STAGES * STAGEB + (size_t)warp * Math::kScratch;
 
     Cursor ahead;
-    ahead.seek(p, lo + skip, lane, first, first_sum);
+    ahead.seek(p, lo + skip, lane, survey);
     Cursor at = ahead;
     bool begins = at.u == at.s.u0;
 
