@@ -90,19 +90,20 @@ class Rotary:
         magnitudes below 2^31.  Channels from rotary_dim on pass unchanged.  Returns the rotated pair (new tensors);
         differentiable in q and k.  (As with every differentiable call: let go of results of eager calls on the same leaves
         before a call and its backward pass are captured into a graph, torch ties the leaves' gradients to the eager stream.)"""
-        lead, device, rotary_dim = q.shape[:-2], q.get_device(), self.rotary_dim
-        assert 1 <= len(lead) <= 2 and k.shape[:-2] == lead and k.shape[-1] == q.shape[-1], \
-            f"q (..., heads, D) and k (..., heads, D) do not go together: {tuple(q.shape)}, {tuple(k.shape)}"
+        qs, ks, device = q.shape, k.shape, q.get_device()
+        lead = len(qs) - 2
+        assert 1 <= lead <= 2 and len(ks) == lead + 2 and ks[0] == qs[0] and ks[lead - 1] == qs[lead - 1] and ks[-1] == qs[-1], \
+            f"q (..., heads, D) and k (..., heads, D) do not go together: {tuple(qs)}, {tuple(ks)}"
         if device < 0:
             _native.require_cuda(q, "q")
-        assert k.dtype == q.dtype, "q and k must have the same dtype"
-        assert rotary_dim <= q.shape[-1] <= 512, \
-            f"head_dim must lie between rotary_dim ({rotary_dim}) and 512, got {q.shape[-1]}"
+        assert k.dtype is q.dtype, "q and k must have the same dtype"
+        assert self.rotary_dim <= qs[-1] <= 512, \
+            f"head_dim must lie between rotary_dim ({self.rotary_dim}) and 512, got {qs[-1]}"
         assert positions.dtype in _POSITION_TYPES, f"positions must be int32 or int64, got {positions.dtype}"
-        if positions.shape != lead:
-            assert positions.shape == lead[-1:], \
-                f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}"
-            positions = positions.expand(lead)
+        if positions.shape != qs[:lead]:
+            assert positions.shape == qs[lead - 1:lead], \
+                f"positions must be {tuple(qs[:lead])} or {tuple(qs[lead - 1:lead])}, got {tuple(positions.shape)}"
+            positions = positions.expand(qs[:lead])
         assert k.get_device() == positions.get_device() == self._device == device, \
             f"k ({k.device}), positions ({positions.device}) and inv_freq ({self.inv_freq.device}) must be on the device of q ({q.device})"
         if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
