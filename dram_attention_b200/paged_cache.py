@@ -4,6 +4,7 @@ attention of one new token per sequence."""
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional
 
 import torch
@@ -22,6 +23,8 @@ class PagedKVCache:
     int32 holds token t of sequence b in page page_table[b, t // page_size]; entries that no token needs are never read.
     `lengths` (n_sequences,) int32 is the number of tokens of every sequence, the new ones of the step among them; 0 marks a
     row of the batch that is not in use.  Both are read on the device, so a captured step follows them from replay to replay.
+    Calls work on the current stream of the pool's device and share nothing but the pool: ordering calls that write and read
+    the same pages on several streams is the caller's.
 
     Args:
         n_pages, page_size: pages in the pool, tokens per page.
@@ -56,15 +59,24 @@ class PagedKVCache:
         assert pages.data_ptr() % 16 == 0 and all(s % piece == 0 for n, s in zip(pages.shape, pages.stride()[:2]) if n > 1), \
             "pages must start on 16-byte boundaries"
         _native.lib()
-        self.pages = pages.detach()
+        self._pages = pages.detach()
         self.n_kv_heads, self.n_pages, self.page_size, _, self.head_dim = pages.shape
         # (the stride of a dimension of one entry is never followed)
         head, page = pages.stride()[:2]
-        self._pool = (self.pages.data_ptr(), page if self.n_pages > 1 else 0, head if self.n_kv_heads > 1 else 0, self.page_size,
-                      self.n_pages)
+        self._layout = (page if self.n_pages > 1 else 0, head if self.n_kv_heads > 1 else 0, self.page_size, self.n_pages)
         self._device, self._dtype, self._dtype_code, self._piece = pages.get_device(), pages.dtype, _native.dtype_code(pages.dtype), piece
         self._scratch = {}
         self.status = torch.zeros(1, dtype=torch.int32, device=pages.device)
+
+    @property
+    def pages(self) -> torch.Tensor:
+        return self._pages
+
+    def __getstate__(self):
+        return {"pages": self._pages}     # (a copied or saved cache works on its own pages)
+
+    def __setstate__(self, state) -> None:
+        self._set_pages(state["pages"])
 
     # ---- checks shared by the calls --------------------------------------------------------
     def _check_heads(self, t: torch.Tensor, name: str, rows: Optional[int], heads: Optional[int]) -> torch.Tensor:
@@ -81,7 +93,7 @@ class PagedKVCache:
 
     def _wrong_device(self, t: torch.Tensor, name: str) -> None:
         _native.require_cuda(t, name)
-        raise AssertionError(f"{name} must be on the device of the pages ({self.pages.device}), got {t.device}")
+        raise AssertionError(f"{name} must be on the device of the pages ({self._pages.device}), got {t.device}")
 
     def _check_table(self, page_table: torch.Tensor, lengths: torch.Tensor):
         """Sequences, columns and row stride of the table"""
@@ -106,12 +118,13 @@ class PagedKVCache:
         """Write the keys and values of new tokens to their pages, the keys rotated by their position when `rotary` is given.
 
         k, v (rows, n_kv_heads, D): without `starts` one row per sequence; with `starts` (n_sequences + 1,) int32, rows
-        starts[b] to starts[b + 1] are the new tokens of sequence b.  `lengths` counts them already: the last
-        new token of sequence b is its token lengths[b] - 1.  Rows in front of and behind the sequences (a padded batch), and those
-        of sequences of length 0, are left out.
+        starts[b] to starts[b + 1] are the new tokens of sequence b (starts does not decrease).  `lengths` counts them already:
+        the last new token of sequence b is its token lengths[b] - 1.  Rows in front of and behind the sequences (a padded
+        batch), and those of sequences of length 0, are left out.
         q (rows, Hq, D), only with `rotary`: returned rotated like the keys (a new tensor; rows left out are zero).
-        Two sequences must not append to the same page.  A position outside the table or a page outside the pool writes
-        nothing and is reported by `check_status`."""
+        No two new tokens may have the same place (two sequences that append to one page, a page listed twice), and k, v and q
+        must not lie in the pool.  A position outside the table or a page outside the pool writes nothing and is reported by
+        `check_status`."""
         n, columns, table_stride = self._check_table(page_table, lengths)
         k = self._check_heads(k, "k", None, self.n_kv_heads)
         rows = k.shape[0]
@@ -128,9 +141,10 @@ class PagedKVCache:
         out, qp, qo, qs, hq, turn = None, 0, 0, (0, 0), 0, (0, 0, 0, 1.0)
         if rotary is not None:
             assert rotary.rotary_dim <= self.head_dim, f"rotary_dim {rotary.rotary_dim} exceeds head_dim {self.head_dim}"
-            if rotary._device != self._device:
-                self._wrong_device(rotary.inv_freq, "inv_freq")
-            turn = (rotary.inv_freq.data_ptr(), rotary.rotary_dim, rotary.interleaved, rotary.factor)
+            inv_freq = rotary.inv_freq
+            if inv_freq.get_device() != self._device:
+                self._wrong_device(inv_freq, "inv_freq")
+            turn = (inv_freq.data_ptr(), rotary.rotary_dim, rotary.interleaved, rotary.factor)
         if q is not None:
             assert rotary is not None, "q is only rotated: pass rotary with it"
             q = self._check_heads(q, "q", rows, None)
@@ -143,7 +157,7 @@ class PagedKVCache:
         if n == 0:
             return None if out is None else out.zero_()
         _native.launch(_native.lib().da_append_pages, _native.PACK_APPEND(
-            qp, k.data_ptr(), v.data_ptr(), qo, *qs, *k.stride()[:2], *v.stride()[:2], *self._pool, page_table.data_ptr(),
+            qp, k.data_ptr(), v.data_ptr(), qo, *qs, *k.stride()[:2], *v.stride()[:2], self._pages.data_ptr(), *self._layout, page_table.data_ptr(),
             table_stride, columns, lengths.data_ptr(), starts_ptr, n, rows, *turn, hq, self.n_kv_heads, self.head_dim,
             self._dtype_code, self.status.data_ptr(), _native.stream_of(self._device)), self._device, "da_append_pages")
         return out
@@ -153,13 +167,19 @@ class PagedKVCache:
         """Attention of one token per sequence, q (n_sequences, Hq, D) with Hq a multiple of n_kv_heads (query head h reads
         KV head h // (Hq / n_kv_heads)), over the first lengths[b] tokens of its sequence, or the last `window` of them.
         Logits are scaled by `scale` (default 1 / sqrt(D)).  Returns (n_sequences, Hq, D); with `return_lse` also the float32
-        log-sum-exp of the scaled logits (n_sequences, Hq).  A sequence of length 0 gives zeros and -inf."""
+        log-sum-exp of the scaled logits (n_sequences, Hq).  A sequence of length 0 gives zeros and -inf.  What pages hold beyond
+        the attended tokens does not matter, NaN and infinities included; attended keys and values are taken to be finite.
+        The same inputs give the same bits.  Tokens in pages outside the pool are left out and lengths outside the
+        table are cut; `check_status` reports both."""
         n, columns, table_stride = self._check_table(page_table, lengths)
         q = self._check_heads(q, "q", n, None)
         hq = q.shape[1]
         rep = hq // self.n_kv_heads
         assert rep > 0 and hq == rep * self.n_kv_heads, f"{hq} query heads do not divide among {self.n_kv_heads} KV heads"
+        window = operator.index(window)
         assert window >= 0, f"window must not be negative, got {window}"
+        if window >= columns * self.page_size:
+            window = 0
         strides = q.stride()
         if q.data_ptr() % 16 or strides[0] % self._piece or strides[1] % self._piece:
             q = q.clone(memory_format=torch.contiguous_format)
@@ -171,7 +191,7 @@ class PagedKVCache:
             size, like = self._scratch.get((n, rep)) or self._scratch_like(n, rep)
             scratch = torch.empty_like(like)
             _native.launch(_native.lib().da_paged_attention, _native.PACK_ATTEND(
-                q.data_ptr(), strides[0], strides[1], *self._pool, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
+                q.data_ptr(), strides[0], strides[1], self._pages.data_ptr(), *self._layout, page_table.data_ptr(), table_stride, columns, lengths.data_ptr(),
                 n, window, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), out.data_ptr(),
                 0 if lse is None else lse.data_ptr(), scratch.data_ptr(), size, self.status.data_ptr(), self.n_kv_heads, rep,
                 self.head_dim, self._dtype_code, _native.stream_of(self._device)), self._device, "da_paged_attention")
@@ -183,12 +203,19 @@ class PagedKVCache:
         size = _native.lib().da_paged_attention_workspace_bytes(n, self.n_kv_heads, rep, self.head_dim, self._dtype_code)
         if len(self._scratch) >= 256:
             self._scratch.clear()
-        entry = self._scratch[n, rep] = (size, torch.empty(1, dtype=torch.uint8, device=self.pages.device).expand(max(size, 16)))
+        entry = self._scratch[n, rep] = (size, torch.empty(1, dtype=torch.uint8, device=self._pages.device).expand(max(size, 16)))
         return entry
 
     def check_status(self) -> None:
-        """Synchronises; raises if any call on this pool flagged a problem."""
+        """Synchronises; raises if any call on this pool flagged a problem since the last check."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
-            raise RuntimeError("dram_attention_b200 device status: " + _native.status_message(bits))
+            raise RuntimeError("dram_attention_b200 device status: " + "; ".join(t for b, t in _STATUS_TEXT.items() if bits & b))
+
+
+_STATUS_TEXT = {
+    _native.STATUS_BAD_PAGE_ID: "a page id in the page table was outside the pool",
+    _native.STATUS_BAD_POSITION: "a length or a position was outside the page table",
+    _native.STATUS_WAIT_TIMEOUT: "a bounded wait on an asynchronous copy ran out",
+}

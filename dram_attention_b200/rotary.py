@@ -67,7 +67,8 @@ class Rotary:
     """Rotary positions with the given inverse frequencies.
 
     Args:
-        inv_freq: float32 (rotary_dim / 2,) on a CUDA device; `rotary_frequencies` makes them.
+        inv_freq: float32 (rotary_dim / 2,) on a CUDA device; `rotary_frequencies` makes them.  Its values may be changed in
+            place between calls, e.g. for frequencies that follow the length.
         factor: amplitude of the rotated channels.
         interleaved: channel pairs (2i, 2i + 1); otherwise (i, i + rotary_dim / 2).
 
@@ -79,11 +80,18 @@ class Rotary:
         assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.numel() > 0, \
             f"inv_freq must be a float32 vector, got {tuple(inv_freq.shape)} {inv_freq.dtype}"
         _native.lib()
-        self.inv_freq = inv_freq.detach().contiguous()
-        self.rotary_dim = 2 * inv_freq.numel()
+        self._inv_freq = inv_freq.detach().contiguous()
+        self._rotary_dim = 2 * inv_freq.numel()
         self.factor = float(factor)
         self.interleaved = bool(interleaved)
-        self._device = inv_freq.get_device()
+
+    @property
+    def inv_freq(self) -> torch.Tensor:
+        return self._inv_freq
+
+    @property
+    def rotary_dim(self) -> int:
+        return self._rotary_dim
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
         """q (s, Hq, D) or (b, s, Hq, D), k the same with its own number of heads; positions int32 or int64, (s,) or (b, s),
@@ -97,18 +105,19 @@ class Rotary:
         if device < 0:
             _native.require_cuda(q, "q")
         assert k.dtype is q.dtype, "q and k must have the same dtype"
-        assert self.rotary_dim <= qs[-1] <= 512, \
+        assert self._rotary_dim <= qs[-1] <= 512, \
             f"head_dim must lie between rotary_dim ({self.rotary_dim}) and 512, got {qs[-1]}"
         assert positions.dtype in _POSITION_TYPES, f"positions must be int32 or int64, got {positions.dtype}"
         if positions.shape != qs[:lead]:
             assert positions.shape == qs[lead - 1:lead], \
                 f"positions must be {tuple(qs[:lead])} or {tuple(qs[lead - 1:lead])}, got {tuple(positions.shape)}"
             positions = positions.expand(qs[:lead])
-        assert k.get_device() == positions.get_device() == self._device == device, \
-            f"k ({k.device}), positions ({positions.device}) and inv_freq ({self.inv_freq.device}) must be on the device of q ({q.device})"
+        inv_freq = self._inv_freq
+        assert k.get_device() == positions.get_device() == inv_freq.get_device() == device, \
+            f"k ({k.device}), positions ({positions.device}) and inv_freq ({inv_freq.device}) must be on the device of q ({q.device})"
         if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
-            return _Rotate.apply(q, k, positions, self.inv_freq, self.factor, self.interleaved, False)
-        return _rotate(q, k, positions, self.inv_freq, self.factor, self.interleaved, False)
+            return _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
+        return _rotate(q, k, positions, inv_freq, self.factor, self.interleaved, False)
 
 
 _POSITION_TYPES = (torch.int32, torch.int64)

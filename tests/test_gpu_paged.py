@@ -398,7 +398,7 @@ def test_bad_pages_and_lengths_are_left_out_and_reported(da):
 
     capacity = 2 * 16
     out = cache.attend(q, table[:, :2].contiguous(), torch.tensor([-3, 64, 30], dtype=torch.int32, device=DEV))
-    with pytest.raises(RuntimeError, match="start_pos|outside"):
+    with pytest.raises(RuntimeError, match="outside the page table"):
         cache.check_status()
     assert bool((out[0] == 0).all())
     want, _, tol, _ = _attention(q[1:2], [keys[1][:, :capacity]], [values[1][:, :capacity]], 0, 0.125)
@@ -419,6 +419,52 @@ def test_attention_of_many_sequences_and_of_none(da):
     out = cache.attend(q, table, torch.zeros_like(n))
     assert bool((out == 0).all())
     cache.check_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_long_sequence_among_many_short_ones(da, dtype):
+    lengths = [3] * 300 + [20000] + [(i * 13) % 40 for i in range(400)]
+    pool, table, keys, values = _pool(10, lengths, 2, 16, 64, dtype)
+    q = _randn(44, len(lengths), 8, 64, dtype=dtype)
+    cache = da.PagedKVCache.over(pool)
+    out, lse = cache.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), return_lse=True)
+    cache.check_status()
+    want, want_lse, tol, tol_lse = _attention(q, keys, values, 0, 0.125)
+    _assert_attended(out, want, tol)
+    some = torch.tensor(lengths, device=DEV) > 0
+    _assert_attended(lse[some], want_lse[some], tol_lse[some])
+
+
+def test_copied_and_saved_caches_work_on_their_own_pages(da):
+    import copy
+    import io
+    cache = da.PagedKVCache(4, 16, 2, 64)
+    table, one = torch.tensor([[2]], dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    k = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    cache.attend(k, table, one)
+    twin = copy.deepcopy(cache)
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    loaded = torch.load(file, weights_only=False)
+    for other in (twin, loaded):
+        other.append_(k, k, table, one)
+        assert bool((other.attend(k, table, one) == 1).all()) and bool((other.pages[:, 2, 0] == 1).all())
+    assert bool((cache.pages == 0).all()) and bool((cache.attend(k, table, one) == 0).all())
+    with pytest.raises(AttributeError):
+        cache.pages = twin.pages
+    r = copy.deepcopy(da.Rotary(_frequencies(64)))
+    assert r.rotary_dim == 64 and r(k[:, :, :], k, one)[0].shape == k.shape
+    with pytest.raises(AttributeError):
+        r.inv_freq = _frequencies(32)
+
+
+def test_frequencies_changed_in_place_are_followed(da):
+    f = _frequencies(64)
+    r = da.Rotary(f)
+    q, p = _randn(45, 5, 2, 64), torch.arange(5, device=DEV)
+    r.inv_freq.mul_(0.5)
+    _assert_turned(r(q, q, p)[0], q, p, _frequencies(64) * 0.5, 1.0, True)
 
 
 def test_pool_of_more_than_2_to_31_elements(da):
@@ -535,7 +581,7 @@ def test_append_skips_what_is_not_in_use_and_reports_what_is_wrong(da):
     # positions outside the table
     cache = da.PagedKVCache.over(pool.clone())
     out = cache.append_(k, v, table, torch.tensor([33, -1, 2 ** 31 - 1, 32], dtype=torch.int32, device=DEV), q=q, rotary=r)
-    with pytest.raises(RuntimeError, match="outside"):
+    with pytest.raises(RuntimeError, match="outside the page table"):
         cache.check_status()
     assert bool((out[:3] == 0).all())
     changed = (cache.pages != pool).flatten(3).any(-1).any(0)
@@ -543,7 +589,7 @@ def test_append_skips_what_is_not_in_use_and_reports_what_is_wrong(da):
     # more new tokens than the sequence has
     cache = da.PagedKVCache.over(pool.clone())
     cache.append_(k, v, table[:1], torch.tensor([2], dtype=torch.int32, device=DEV), starts=torch.tensor([0, 4], dtype=torch.int32, device=DEV))
-    with pytest.raises(RuntimeError, match="outside"):
+    with pytest.raises(RuntimeError, match="outside the page table"):
         cache.check_status()
     changed = (cache.pages != pool).flatten(3).any(-1).any(0)
     assert changed.nonzero().tolist() == [[0, 0], [0, 1]]
@@ -587,6 +633,9 @@ def test_paged_calls_refuse(da):
             bad()
     with pytest.raises(RuntimeError, match="outside"):
         cache.attend(_randn(3, 3, 2 * 300, 64, dtype=torch.bfloat16), table, n)      # more queries to a key than the kernels take
+    with pytest.raises(TypeError):
+        cache.attend(q, table, n, window=1.5)
+    cache.attend(q, table, n, window=2 ** 62)
     with torch.no_grad():
         cache.attend(q.clone().requires_grad_(), table, n)
     cache.check_status()
