@@ -124,6 +124,15 @@ __device__ __forceinline__ void turn(float &a, float &b, float2 cs) {
     b = y;
 }
 
+// The last sequence that does not begin behind a row, or -1; by a warp, all starts at once.
+__device__ __forceinline__ int find_near(const RotateParams &p, int row, int lane) {
+    int count = 0;
+    for (int i = lane; i <= p.n_sequences; i += 32) count += __ldg(p.starts + i) <= row;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) count += __shfl_xor_sync(DA_FULL_MASK, count, off);
+    return count - 1;
+}
+
 // Where a row of the ragged batch belongs.
 struct Place {
     long long position;
@@ -132,20 +141,21 @@ struct Place {
     bool used;                // the row belongs to a sequence and its position exists
     int status;
 };
-__device__ __forceinline__ Place find_place(const RotateParams &p, int row) {
+// `near`: a sequence that does not begin behind the row (the one of the block's first row, or -1).
+__device__ __forceinline__ Place find_place(const RotateParams &p, int row, int near) {
     Place at = {0, -1, 0, false, 0};
     int b = row, first = row, n_new = 1;
     if (p.starts) {
-        int lo = 0, hi = p.n_sequences + 1;     // how many starts are <= row
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (__ldg(p.starts + mid) <= row) lo = mid + 1;
-            else hi = mid;
+        b = near;
+        int next = b < p.n_sequences ? __ldg(p.starts + b + 1) : 0;
+        first = b >= 0 ? __ldg(p.starts + b) : 0;
+        while (b < p.n_sequences && next <= row) {           // the row belongs to a sequence further on
+            first = next;
+            ++b;
+            next = b < p.n_sequences ? __ldg(p.starts + b + 1) : 0;
         }
-        b = lo - 1;
         if (b < 0 || b >= p.n_sequences) return at;          // a row in front of or behind the sequences
-        first = __ldg(p.starts + b);
-        n_new = __ldg(p.starts + b + 1) - first;
+        n_new = next - first;
     }
     const int length = __ldg(p.lengths + b);
     if (length == 0) return at;                              // an entry of the batch that is not in use
@@ -172,15 +182,15 @@ __device__ __forceinline__ Place find_place(const RotateParams &p, int row) {
 //                 (2000 tokens of 16 + 4 heads, 17 pairs: channel by channel 44 us instead of 12)
 enum Pairing { kNeighbours, kHalves, kCrossed };
 
-// (three blocks of 384 threads on an SM: with a few registers more it is two, and a 32K append takes 147 us instead of 126)
 template <typename T, int V, Pairing PAIRING, bool PAGED>
-__global__ void __launch_bounds__(V > 1 ? 384 : 512, V > 1 ? (PAIRING == kNeighbours ? 3 : 2) : 1)
+__global__ void __launch_bounds__(V > 1 ? 256 : 512, V > 1 ? (PAIRING == kNeighbours ? 4 : 3) : 1)
 rotate_kernel(const RotateParams p) {
     constexpr bool HALF = PAIRING == kHalves, CROSSED = PAIRING == kCrossed;
     constexpr bool kTwo = HALF || (V == 1 && !CROSSED);          // a rotating column has two chunks
     constexpr int kPairs = kTwo || CROSSED ? V : V / 2;          // pairs it takes part in
     extern __shared__ float2 cos_sin[];           // [tokens of the block][rot_half]
     __shared__ double sh_position[kRotateTokens];
+    __shared__ int sh_near;
     __shared__ long long sh_place[PAGED ? kRotateTokens : 1];   // offset in the pool, -1: no page, -2: a row of no sequence
     griddep_wait();
     griddep_launch_dependents();
@@ -231,10 +241,21 @@ rotate_kernel(const RotateParams p) {
     request(z);
 
     // the tokens' positions and places, while the first rows are on their way
+    if constexpr (PAGED) {
+        if (p.starts) {
+            if (linear < 32 && threads >= 32) {
+                const int near = find_near(p, first, linear);
+                if (linear == 0) sh_near = near;
+            } else if (threads < 32 && linear == 0) {
+                sh_near = -1;                      // (a walk from the front)
+            }
+            __syncthreads();
+        }
+    }
     if (linear < here) {
         const int t = first + linear;
         if constexpr (PAGED) {
-            const Place at = find_place(p, t);
+            const Place at = find_place(p, t, p.starts ? sh_near : 0);
             if (at.status && blockIdx.y == 0) atomicOr(p.status, at.status);
             sh_position[linear] = (double)at.position;
             sh_place[linear] = !at.used ? -2 : (at.page < 0 ? -1 : at.page * p.page_stride + (long long)at.slot * 2 * p.head_dim);
@@ -339,12 +360,11 @@ static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
             if (best < 0 || places * 8 < best * 7) best = places, p.rows_each = each;
         }
     }
-    // Whole tokens up to the size of a block.  Small blocks and one token per thread are fastest (32 768 tokens of 32 + 8 heads in
-    // halves: 105 us with blocks of 96 to 192 threads, 115 with 384; two tokens in turn 127), but for an append whose columns are one
-    // chunk: the look-up of the places is then worth sharing (32 768 tokens: 126 us with 384 threads and two tokens in turn,
-    // 136 with 128 and one).
-    constexpr bool kShare = PAGED && PAIRING == kNeighbours && V > 1;
-    constexpr int THREADS = kShare ? 384 : 128;
+    // Whole tokens up to the size of a block; small blocks are fastest (32 768 tokens of 32 + 8 heads in halves: 105 us with 96 to
+    // 192 threads, 115 with 384).  Then a few tokens in turn, which share the look-ups and angles of a block (append of 32 768
+    // tokens of 32 + 8 heads in neighbours: 143 us with one, 131 with four; of 59 000 of 4 + 1: 43 and 31), unless a thread has
+    // eight chunks under way already (19 000 tokens of 32 + 8 heads in halves: 82 us with one, 95 with four).
+    constexpr int THREADS = 128;
     const int all_y = threads_for(p.rows_each);
     int y = columns * all_y <= 192 ? all_y : THREADS / columns;   // (the angles of a token are made once, then)
     if (y < 1) y = 1;
@@ -354,7 +374,11 @@ static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     if (z > kRotateTokens / 2) z = kRotateTokens / 2;
     while (z > 1 && p.all_tokens / z < 148) z >>= 1;
     if (z < 1) z = 1;
-    const int rounds = kShare && p.all_tokens / z >= 2 * 8 * 148 ? 2 : 1;
+    constexpr int CHUNKS = PAIRING == kHalves || (V == 1 && PAIRING == kNeighbours) || PAIRING == kCrossed ? 2 : 1;
+    int rounds = p.rows_each * CHUNKS <= 4 ? p.all_tokens / (z * 16 * 148) : 1;
+    if (rounds > 4) rounds = 4;
+    if (rounds > kRotateTokens / z) rounds = kRotateTokens / z;
+    if (rounds < 1) rounds = 1;
     p.rounds = rounds;
     const int per_block = z * rounds;
     return (int)launch_dependent(rotate_kernel<T, V, PAIRING, PAGED>, dim3((unsigned)(((long long)p.all_tokens + per_block - 1) / per_block), blocks_y),
