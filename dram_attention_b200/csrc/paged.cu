@@ -1,4 +1,4 @@
-// Attention over a paged cache: the join of the items that cross CTAs, and the host side.
+// Attention over a paged cache: the join of the items that cross warps, and the host side.
 
 #include "paged_attn.cuh"
 
@@ -214,7 +214,7 @@ extern "C" int da_paged_attention(const da_paged_attention_args *args) {
     if (!a.q || !a.pages || !a.page_table || !a.lengths || !a.out || !a.workspace || !a.status) return DA_ERR_NULL;
     if (a.dtype < DA_F32 || a.dtype > DA_BF16) return DA_ERR_DTYPE;
     if (a.n_sequences < 1 || a.n_kv_heads < 1 || a.rep < 1 || a.page_size < 1 || a.n_pages < 1 || a.table_columns < 1 ||
-        a.window < 0 || a.n_sequences > 0x7fffffff || a.n_kv_heads > 1 << 16 || a.page_size > 1 << 20 || a.n_pages > 0x7fffffff ||
+        a.window < 0 || a.n_sequences > 0x7fffffff || a.n_kv_heads > 1 << 16 || a.page_size > 1 << 30 || a.n_pages > 0x7fffffff ||
         a.table_columns > 0x7fffffff || a.table_columns * a.page_size > 0x7fffff00 || a.window > 0x7fffffff)
         return DA_ERR_SHAPE;
     if (!paged_shape(a.rep, a.head_dim, a.dtype)) return DA_ERR_UNSUPPORTED;

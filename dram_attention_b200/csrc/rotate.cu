@@ -4,9 +4,9 @@
 //   of the rotated part); the channels behind the rotated part are copied.  The gradient of x is the rotation back,
 //   factor * R(-p * w_i) dy: the same kernel with the sign of the angle turned.
 //
-// The angle p * w_i is taken in turns and in 64 bits, reduced there to an eighth of a turn either way, and only then
-// rounded: at position 1 000 000 a 32-bit product is off by up to 0.03 rad, this one by 3e-8 at any position.  Products and
-// sums are 32-bit, the result is rounded once to the element type.
+// The angle p * w_i is taken in quarter turns and in 64 bits, reduced there to an eighth of a turn either way, and only then
+// rounded: at position 1 000 000 a 32-bit product is off by up to 0.03 rad, this one by 3e-8 up to position 10^8 (and by 5e-7 at
+// 2^31, where 64 bits end).  Products and sums are 32-bit, the result is rounded once to the element type.
 //
 // Bound by memory: a token of 32 + 8 heads of 128 bf16 channels is 10 KB in and 10 KB out against 64 angles.  What stands in the
 // way is the number of instructions, so a thread keeps its place: one column of up to four neighbouring heads, for several
@@ -179,7 +179,7 @@ __device__ __forceinline__ Place find_place(const RotateParams &p, int row, int 
 //   kNeighbours   channel 2 i is paired with 2 i + 1: one chunk of V channels, whole pairs (V 1: the two channels of a pair)
 //   kHalves       channel i is paired with i + rot / 2, a multiple of V: the chunks of both members
 //   kCrossed      the same where rot / 2 is no multiple of V: one chunk, the other members of its pairs read one by one
-//                 (2000 tokens of 16 + 4 heads, 17 pairs: channel by channel 44 us instead of 12)
+//                 (8000 tokens of 16 + 4 heads of 80, 17 pairs: channel by channel 44 us, so 28)
 enum Pairing { kNeighbours, kHalves, kCrossed };
 
 template <typename T, int V, Pairing PAIRING, bool PAGED>
@@ -252,17 +252,17 @@ rotate_kernel(const RotateParams p) {
             __syncthreads();
         }
     }
-    if (linear < here) {
-        const int t = first + linear;
+    for (int j = linear; j < here; j += threads) {
+        const int t = first + j;
         if constexpr (PAGED) {
             const Place at = find_place(p, t, p.starts ? sh_near : 0);
             if (at.status && blockIdx.y == 0) atomicOr(p.status, at.status);
-            sh_position[linear] = (double)at.position;
-            sh_place[linear] = !at.used ? -2 : (at.page < 0 ? -1 : at.page * p.page_stride + (long long)at.slot * 2 * p.head_dim);
+            sh_position[j] = (double)at.position;
+            sh_place[j] = !at.used ? -2 : (at.page < 0 ? -1 : at.page * p.page_stride + (long long)at.slot * 2 * p.head_dim);
         } else {
             const int n = t / p.position_tokens;
             const long long i = n * p.position_batch + (t - n * p.position_tokens) * p.position_token;
-            sh_position[linear] = p.positions_64 ? (double)__ldg(static_cast<const long long *>(p.positions) + i)
+            sh_position[j] = p.positions_64 ? (double)__ldg(static_cast<const long long *>(p.positions) + i)
                                                  : (double)__ldg(static_cast<const int32_t *>(p.positions) + i);
         }
     }
@@ -374,7 +374,7 @@ static int launch_rotate(RotateParams p, int n_batch, cudaStream_t stream) {
     if (z > kRotateTokens / 2) z = kRotateTokens / 2;
     while (z > 1 && p.all_tokens / z < 148) z >>= 1;
     if (z < 1) z = 1;
-    constexpr int CHUNKS = PAIRING == kHalves || (V == 1 && PAIRING == kNeighbours) || PAIRING == kCrossed ? 2 : 1;
+    constexpr int CHUNKS = PAIRING == kNeighbours && V > 1 ? 1 : 2;
     int rounds = p.rows_each * CHUNKS <= 4 ? p.all_tokens / (z * 16 * 148) : 1;
     if (rounds > 4) rounds = 4;
     if (rounds > kRotateTokens / z) rounds = kRotateTokens / z;
@@ -474,7 +474,7 @@ extern "C" int da_append_pages(const da_append_pages_args *args) {
     if (!small(a.dtype, DA_F32, DA_BF16)) return DA_ERR_DTYPE;
     if (!small(a.n_rows, 1, 1 << 30) || !small(a.n_sequences, 1, 1 << 30) || (!a.starts && a.n_rows != a.n_sequences) ||
         !small(a.head_dim, 2, 512) || (a.q && !small(a.n_q_heads, 1, 1 << 14)) || !small(a.n_kv_heads, 1, 1 << 14) ||
-        !small(a.page_size, 1, 1 << 20) || !small(a.n_pages, 1, 0x7fffffff) || !small(a.table_columns, 1, 0x7fffffff) ||
+        !small(a.page_size, 1, 1 << 30) || !small(a.n_pages, 1, 0x7fffffff) || !small(a.table_columns, 1, 0x7fffffff) ||
         a.table_columns * a.page_size > 0x7fffff00 ||
         (a.inv_freq && (!small(a.rotary_dim, 2, a.head_dim) || (a.rotary_dim & 1))))
         return DA_ERR_SHAPE;

@@ -96,6 +96,17 @@ def test_rotation_at_far_positions(da, interleaved):
     _assert_turned(k2, k, positions, f, 1.0, interleaved)
 
 
+@pytest.mark.parametrize("d,tokens", [(8, 200003), (2, 100001), (64, 70001)])
+def test_rotation_of_many_tokens_with_few_channels(da, d, tokens):
+    f = _frequencies(d)
+    positions = torch.arange(tokens, device=DEV, dtype=torch.int32)
+    q, k = _randn(46, tokens, 1, d, dtype=torch.bfloat16), _randn(47, tokens, 1, d, dtype=torch.bfloat16)
+    for interleaved in (True, False):
+        q2, k2 = da.Rotary(f, interleaved=interleaved)(q, k, positions)
+        _assert_turned(q2, q, positions, f, 1.0, interleaved)
+        _assert_turned(k2, k, positions, f, 1.0, interleaved)
+
+
 def test_rotation_equals_the_table_form(da):
     """The operator's own rotation (complex factors of the whole head) and this one agree to the bound."""
     f = _frequencies(128)
@@ -483,6 +494,23 @@ def test_pool_of_more_than_2_to_31_elements(da):
     part = lambda x: [x[:40].transpose(0, 1).double(), x[40:].transpose(0, 1).double()]
     want, _, tol, _ = _attention(q, part(k), part(v), 0, 0.125)
     _assert_attended(out, want, tol)
+
+
+def test_page_of_more_than_a_million_tokens(da):
+    """A contiguous cache per sequence is one page."""
+    page, n = 1500001, 1499990
+    pool = torch.empty(1, 2, page, 2, 256, dtype=torch.float16, device=DEV)
+    k, v = _randn(48, 1, 300, 256, dtype=torch.float16), _randn(49, 1, 300, 256, dtype=torch.float16)
+    pool[0, 1, n - 300:n, 0], pool[0, 1, n - 300:n, 1] = k[0], v[0]
+    cache = da.PagedKVCache.over(pool)
+    table, lengths = torch.tensor([[1]], dtype=torch.int32, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = _randn(50, 1, 4, 256, dtype=torch.float16)
+    out = cache.attend(q, table, lengths, window=300)
+    cache.check_status()
+    want, _, tol, _ = _attention(q, [k.double()], [v.double()], 0, 256 ** -0.5)
+    _assert_attended(out, want, tol)
+    cache.append_(k.transpose(0, 1), v.transpose(0, 1), table, lengths + 5, starts=torch.tensor([0, 300], dtype=torch.int32, device=DEV))
+    assert torch.equal(pool[0, 1, n - 295:n + 5, 0], k[0])
 
 
 # ----------------------------------------------------------------- append -----
