@@ -15,7 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libdram_attention_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["api.cu", "score.cu", "topk.cu", "lru.cu", "fetch.cu", "gather.cu", "rope.cu", "prefill.cu", "attn.cu", "attn_mma.cu",
-           "step.cu", "rotate.cu", "paged.cu", "paged_f32.cu", "paged_f16.cu", "paged_bf16.cu"]
+           "step.cu", "rotate.cu", "rotate_f32.cu", "rotate_f16.cu", "rotate_bf16.cu", "paged.cu",
+           "paged_f32.cu", "paged_f16.cu", "paged_bf16.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
