@@ -162,13 +162,15 @@ template <typename T, int D> static cudaError_t launch_join(const PagedParams &p
     constexpr int ALL = D / 4, NARROW = D % 32 == 0 ? 8 : 4, BLOCKS = ALL / NARROW;
     const long long items = (long long)p.n_sequences * p.n_kv_heads * p.groups, rows = items * p.group_rows;
     const unsigned x = (unsigned)items;
-    // A CTA per row as long as all of them are on the GPU at once, of 1024 threads (with narrow columns if even then) or of 256;
-    // then a warp (16 sequences of 200 tokens, 512 rows: 9.9 against 13.6 us; 32 of 1000, 2048 rows: 33.9 against 28.3).
-    if (rows * BLOCKS <= 2 * kPagedCtas)
+    // CTAs of 1024 threads, narrow columns, while no SM gets two of them: few rows are of many parts (100 000 tokens of one head,
+    // sixteen rows: 19.5 us, with 256 threads 24.8).  Up to a row for every SM CTAs of 256 with narrow columns (two of 2000 with 8
+    // heads, 64 rows: 10.5, with 1024 threads 14.9), then with all columns while four lie on an SM (6 of 2000, 192 rows: 15.2,
+    // narrow 18.4), then a warp per row (32 of 1000 with 8 heads, 768 to 1024 rows: 2 to 3 us less than a CTA per row; 512 rows 1 to 2 more).
+    if (rows * BLOCKS <= kPagedCtas)
         return launch_dependent(paged_join_kernel<T, D, 32, NARROW, false>, dim3(x, p.group_rows, BLOCKS), dim3(1024), (size_t)0, stream, p);
-    if (rows <= 2 * kPagedCtas)
-        return launch_dependent(paged_join_kernel<T, D, 32, ALL, false>, dim3(x, p.group_rows), dim3(1024), (size_t)0, stream, p);
-    if (rows <= 8 * kPagedCtas)
+    if (rows <= kPagedCtas)
+        return launch_dependent(paged_join_kernel<T, D, 8, NARROW, false>, dim3(x, p.group_rows, BLOCKS), dim3(256), (size_t)0, stream, p);
+    if (rows <= 4 * kPagedCtas)
         return launch_dependent(paged_join_kernel<T, D, 8, ALL, false>, dim3(x, p.group_rows), dim3(256), (size_t)0, stream, p);
     return launch_dependent(paged_join_kernel<T, D, 8, ALL, true>, dim3((unsigned)((rows + 7) / 8)), dim3(256), (size_t)0, stream, p);
 }
