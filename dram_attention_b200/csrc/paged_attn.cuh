@@ -10,10 +10,10 @@
 // a contiguous stretch of that.  Whatever the lengths are, no warp has more than one unit more than another, and
 // nothing about them has to be known on the host: every warp finds its place from the lengths itself, so a captured launch
 // stays right while the sequences grow.  A warp walks its stretch with a private ring of stages (one mbarrier each) that
-// bulk copies (TMA) fill, one per token: its key and value rows are contiguous in the page.  The ring runs on across the
+// bulk copies (TMA) fill, one for one or more tokens: key and value rows of a token, and tokens, are contiguous in the page.  The ring runs on across the
 // borders of items; there is no barrier of the CTA.  Where a unit lies in one page a single elected lane
 // issues its copies: a bulk copy takes its operands from the warp, so one per lane is a loop over the lanes (60 sequences of 3000
-// tokens, 64 channels: 76 us, elected 64).  16-byte asynchronous copies of all lanes need fewer instructions still but
+// tokens, 64 channels: 76 us, elected 64, two tokens to a copy 61).  16-byte asynchronous copies of all lanes need fewer instructions still but
 // bring in less (64 sequences of 5000 tokens, 128 channels: 221 us against 197).
 //
 // An item that lies in one warp's stretch is written by the warp.  Of one that does not, every warp leaves its partial result (row
@@ -274,14 +274,15 @@ template <typename T> __device__ __forceinline__ void store_divided(T *dst, cons
     }
 }
 
-// Math: the arithmetic of a unit.  kD, kPitch (bytes of a token in shared memory), kScratch (bytes of a warp's own), State, begin
+// Math: the arithmetic of a unit.  kD, kStageBytes (of a unit in shared memory), offset (of a token in it), kTogether (tokens that
+// follow one another there without a gap), kScratch (bytes of a warp's own), State, begin
 // (query rows), consume (one unit), publish (a partial result), write (a complete one).
 template <class Math, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const PagedParams p) {
     using T = typename Math::Elem;
     constexpr int D = Math::kD, PW = PagedRow<D>::kWidth;
     constexpr int ROWB = D * (int)sizeof(T), TOKB = 2 * ROWB;
-    constexpr int STAGEB = kPagedUnit * Math::kPitch;
+    constexpr int STAGEB = Math::kStageBytes;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t bars[WARPS][STAGES];
     __shared__ uint32_t masks[WARPS][STAGES];      // tokens of the unit that are there
@@ -346,12 +347,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             if (elect_one()) {
                 masks[warp][s] = 0xffffu;
                 mbar_arrive_expect_tx(bar, kPagedUnit * TOKB);
-                if constexpr (Math::kPitch == TOKB) {
-                    bulk_copy_g2s_hint(dst, src, kPagedUnit * TOKB, bar, policy);
-                } else {
 #pragma unroll
-                    for (int t = 0; t < kPagedUnit; ++t) bulk_copy_g2s_hint(dst + t * Math::kPitch, src + t * TOKB, TOKB, bar, policy);
-                }
+                for (int t = 0; t < kPagedUnit; t += Math::kTogether)
+                    bulk_copy_g2s_hint(dst + Math::offset(t), src + t * TOKB, Math::kTogether * TOKB, bar, policy);
             }
             __syncwarp();
         } else {
@@ -361,7 +359,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             }
             __syncwarp();
             if (p.whole) src += lane * TOKB;
-            if (lane < kPagedUnit && ((there >> lane) & 1)) bulk_copy_g2s_hint(dst + lane * Math::kPitch, src, TOKB, bar, policy);
+            if (lane < kPagedUnit && ((there >> lane) & 1)) bulk_copy_g2s_hint(dst + Math::offset(lane), src, TOKB, bar, policy);
         }
     };
 
@@ -401,7 +399,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             for (int k = lane; k < kPagedUnit * (ROWB / 16); k += 32) {
                 const int t = k / (ROWB / 16);
                 if (!((mask >> t) & 1))
-                    *reinterpret_cast<uint4 *>(unit + t * Math::kPitch + ROWB + (k % (ROWB / 16)) * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(unit + Math::offset(t) + ROWB + (k % (ROWB / 16)) * 16) = make_uint4(0, 0, 0, 0);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stage's next copies come after
             __syncwarp();
@@ -443,7 +441,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
 
 template <class Math, int WARPS, int STAGES>
 static cudaError_t launch_paged(const PagedParams &p, cudaStream_t stream) {
-    constexpr int SMEM = WARPS * (STAGES * kPagedUnit * Math::kPitch + Math::kScratch);
+    constexpr int SMEM = WARPS * (STAGES * Math::kStageBytes + Math::kScratch);
     static_assert(SMEM <= 224 * 1024, "");
     auto kernel = paged_attention_kernel<Math, WARPS, STAGES>;
     static bool ready[64] = {};

@@ -15,7 +15,8 @@ template <int D_, int R>
 struct PagedSimt {
     using Elem = float;
     static constexpr int kD = D_, kRows = R;
-    static constexpr int ROWB = kD * 4, kPitch = 2 * ROWB;
+    static constexpr int ROWB = kD * 4, kPitch = 2 * ROWB, kTogether = kPagedUnit, kStageBytes = kPagedUnit * kPitch;
+    __device__ __forceinline__ static constexpr int offset(int t) { return t * kPitch; }
     static constexpr int PIECES = kD / 4, NC = (PIECES + 7) / 8;
 
     static constexpr bool kInRegisters = R * NC <= 8;

@@ -5,7 +5,9 @@
 //   S = Q K^T   A = query rows in registers, B = key rows by ldmatrix
 //   O += P V    A = the weights, straight from S's accumulators, B = value rows by ldmatrix.trans
 // A token's rows lie 16 bytes apart from a multiple of 128 bytes in shared memory, so that the eight row addresses of an
-// ldmatrix tile fall into distinct banks for every head size that is a multiple of 16.
+// ldmatrix tile fall into distinct banks for every head size that is a multiple of 16.  Two tokens to a gap halve the number of
+// copies and have two rows in the same banks: faster for 64 channels (64 sequences of 16 000 tokens, 2 heads: 88 us, so 84) and 256
+// (64 of 5000: 123, so 116), slower between them (60 of 3000, 8 heads of 80 and 96: 74 and 86 us, 79 and 93; 128 channels equal).
 #pragma once
 
 #include "mma_sync.cuh"
@@ -13,14 +15,18 @@
 
 namespace da {
 
+constexpr int paged_mma_together(int head_dim) { return head_dim == 64 || head_dim == 256 ? 2 : 1; }
+constexpr int paged_mma_stage(int head_dim) { return kPagedUnit * 4 * head_dim + kPagedUnit / paged_mma_together(head_dim) * 16; }
+
 // FULL: up to 16 query rows; otherwise up to 8 (rows 8..15 of the tile are zero and nothing is kept of them).
 template <typename T, int D_, bool FULL>
 struct PagedMma {
     using Elem = T;
     static constexpr int kD = D_, kRows = FULL ? 16 : 8;
-    static constexpr int ROWB = kD * 2, kPitch = 2 * ROWB + 16;
+    static constexpr int ROWB = kD * 2, kTogether = paged_mma_together(kD), kStageBytes = paged_mma_stage(kD);
     static constexpr int KSTEPS = kD / 16, NT = kD / 8, NR = FULL ? 2 : 1;
     static constexpr int kScratch = 0;
+    __device__ __forceinline__ static constexpr int offset(int t) { return t * 2 * ROWB + t / kTogether * 16; }
     static_assert(kD % 16 == 0, "whole k-steps");
 
     struct State {
@@ -57,9 +63,9 @@ struct PagedMma {
     __device__ __forceinline__ static void consume(State &st, const unsigned char *unit, uint32_t mask, int lane, float scale_log2) {
         const int qd = lane & 3, tile = lane >> 3, tr = lane & 7;
         // key tiles of a k-step: tokens 0..7 and 8..15, channels 0..7 and 8..15 of it
-        const unsigned char *keys = unit + ((tile >> 1) * 8 + tr) * kPitch + (tile & 1) * 16;
+        const unsigned char *keys = unit + offset((tile >> 1) * 8 + tr) + (tile & 1) * 16;
         // value tiles of 16 channels, transposed by the load
-        const unsigned char *values = unit + ROWB + ((tile & 1) * 8 + tr) * kPitch + (tile >> 1) * 16;
+        const unsigned char *values = unit + ROWB + offset((tile & 1) * 8 + tr) + (tile >> 1) * 16;
 
         float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
         float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};   // odd k-steps: four chains instead of two
@@ -165,10 +171,10 @@ struct PagedMma {
 // As many stages as fit for the number of warps that is fastest, but two for 128 channels: 135 KB under way on every SM are enough
 // (64 sequences of 5000 tokens, 1.3 GB: eight warps of three or two stages 206 us, seven of three 211, ten or twelve of two 211,
 // whose threads have too few registers).  Smaller heads have units of fewer bytes, so more of them have to be worked on at a
-// time: twelve (60 sequences of 3000 tokens with 64, 80, 96 channels: 64, 76, 89 us, with eight warps 80 to 100).  The
+// time: twelve (60 sequences of 3000 tokens with 64, 80, 96 channels: 61, 74, 86 us, with eight warps 80 to 100).  The
 // accumulators of 256 channels leave registers for six (265 us; with four warps of three stages 289).
 template <int D> struct PagedMmaShape {
-    static constexpr int kStage = kPagedUnit * (4 * D + 16);
+    static constexpr int kStage = paged_mma_stage(D);
     static constexpr int kWarps = paged_mma_warps(D);
     static constexpr int kStages = D == 128 ? 2 : (220 * 1024) / (kWarps * kStage);
     static_assert(kStages >= 2, "");
