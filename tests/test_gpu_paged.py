@@ -329,6 +329,33 @@ def test_attention(da, dtype, d, hk, rep, page, lengths):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("batch,hk,rep,long", [
+    (1, 2, 3, 9000),      # few rows, each in hundreds of parts
+    (9, 3, 5, 2100),      # 135 rows
+    (16, 4, 5, 900),      # 320
+    (40, 4, 4, 500),      # 640
+    (5, 7, 17, 600),      # rows in several groups, 595 of them
+])
+def test_attention_with_few_rows_and_many(da, dtype, d, batch, hk, rep, long):
+    """The number of rows decides how the parts of an item are joined; lengths from none to long, so that items have from one part to many."""
+    lengths = [(long, 0, 17, long // 2, 1, long // 3)[i % 6] for i in range(batch)]
+    pool, table, keys, values = _pool(91, lengths, hk, 16, d, dtype)
+    q = _randn(92, batch, hk * rep, d, dtype=dtype)
+    cache = da.PagedKVCache.over(pool)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    out, lse = cache.attend(q, table, n, return_lse=True)
+    cache.check_status()
+    want, want_lse, tol, tol_lse = _attention(q, keys, values, 0, d ** -0.5)
+    _assert_attended(out, want, tol)
+    empty = n == 0
+    assert bool((out[empty] == 0).all()) and bool((lse[empty] == -float("inf")).all())
+    _assert_attended(lse[~empty], want_lse[~empty], tol_lse[~empty])
+    again, lse_again = cache.attend(q, table, n, return_lse=True)
+    assert torch.equal(again, out) and torch.equal(lse_again, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window", [1, 15, 16, 100, 513, 10 ** 6])
 @pytest.mark.parametrize("page", [16, 24])
 def test_attention_in_a_window(da, dtype, window, page):
