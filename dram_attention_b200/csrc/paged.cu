@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParam
             for (int off = COLS; off < GROUPS * COLS; off <<= 1) sum.x[0].add_lane(off);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (lane + 32 * i < COLS) store_divided(out + 4 * (lane + 32 * i), sum.x[i].o, sum.x[i].l);
+                if (lane + 32 * i < COLS) store_divided(out + 4 * (lane + 32 * i), sum.x[i].o, sum.x[i].m, sum.x[i].l);
             if (lane == 0 && writes_lse) p.lse[index] = natural_lse(sum.x[0].m, sum.x[0].l);
         }
         if (!__syncthreads_or(n > FEW)) return;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const PagedParam
             float o = 0.f;
 #pragma unroll
             for (int i = 0; i < WARPS; ++i) o = fmaf(sh_o[i][min(c, COLS * 4 - 1)], __shfl_sync(DA_FULL_MASK, k, i), o);
-            if (c < COLS * 4) out[c] = from_float<T>(l > 0.f ? o / l : 0.f);
+            if (c < COLS * 4) out[c] = from_float<T>(m == -INFINITY ? 0.f : o / l);
             if (c == 0 && writes_lse) p.lse[index] = natural_lse(m, l);
         }
     }

@@ -228,6 +228,9 @@ __device__ __forceinline__ int rows_of(const PagedParams &p, int item) {
     return min(p.group_rows, p.rep - (item % p.groups) * p.group_rows);
 }
 __device__ __forceinline__ float natural_lse(float m, float l) { return (m + log2f(l)) * 0.6931471805599453f; }
+// A row's maximum is -inf as long as it has no token, and at least kLowest from then on, were all its logits -inf.  So only a row
+// without tokens is zeros; a weight sum of 0 (every logit -inf) or NaN (a query, or a logit, that is no number) makes the quotient NaN.
+constexpr float kLowest = -3.402823466e38f;
 
 // Running sum of partial results (max, weight sum, four accumulator columns), several at a time so that their loads and
 // exponentials do not wait for one another.
@@ -261,11 +264,11 @@ __device__ __forceinline__ void PartialSum::add_lane(int off) {
     add(ml, v);
 }
 
-// Four consecutive elements, divided by the weight sum.
-template <typename T> __device__ __forceinline__ void store_divided(T *dst, const float4 &o, float l) {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+// Four consecutive elements of a row, divided by its weight sum.
+template <typename T> __device__ __forceinline__ void store_divided(T *dst, const float4 &o, float m, float l) {
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(dst) = l > 0.f ? make_float4(o.x / l, o.y / l, o.z / l, o.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4 *>(dst) = m == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
     } else {
         union { T t[4]; uint2 w; } x;
         x.t[0] = from_float<T>(o.x * inv), x.t[1] = from_float<T>(o.y * inv);
@@ -276,7 +279,7 @@ template <typename T> __device__ __forceinline__ void store_divided(T *dst, cons
 
 // Math: the arithmetic of a unit.  kD, kStageBytes (of a unit in shared memory), offset (of a token in it), kTogether (tokens that
 // follow one another there without a gap), kScratch (bytes of a warp's own), State, begin
-// (query rows), consume (one unit), publish (a partial result), write (a complete one).
+// (query rows), consume (one unit), attended (there was a token), publish (a partial result), write (a complete one).
 template <class Math, int WARPS, int STAGES>
 __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const PagedParams p) {
     using T = typename Math::Elem;
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
     int rows = rows_of(p, id);
     Math::begin(st, p, at.b, at.head, at.group, rows, lane, scratch);
     int s = 0;
-    uint32_t parity = 0;
+    uint32_t parity = 0, seen = 0;                 // seen: tokens of the item this warp has had, by their place in a unit
     for (int i = 0; i < count; ++i) {
         if (issued < count) locate(ahead);
         const bool arrived = mbar_wait_bounded(&bars[warp][s], parity);
@@ -404,6 +407,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stage's next copies come after
             __syncwarp();
         }
+        seen |= mask;
         Math::consume(st, unit, mask, lane, p.scale_log2);
         __syncwarp();
         if (issued < count) {
@@ -424,6 +428,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             if (begins) p.spans[id].x = blockIdx.x * WARPS + warp;
             if (ends) p.spans[id].y = blockIdx.x * WARPS + warp;
         }
+        if (seen) Math::attended(st);
         if (begins && ends) {
             Math::write(st, p, id, rows, lane);
         } else {
@@ -434,6 +439,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Pa
             id = at.id(p);
             rows = rows_of(p, id);
             begins = true;
+            seen = 0;
             Math::begin(st, p, at.b, at.head, at.group, rows, lane, scratch);
         }
     }

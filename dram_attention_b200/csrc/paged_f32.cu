@@ -175,6 +175,8 @@ struct PagedSimt {
         }
     }
 
+    __device__ __forceinline__ static void attended(State &st) { st.m = fmaxf(st.m, kLowest); }
+
     __device__ __forceinline__ static void publish(State &st, float *dst, int lane, int rows) {
         constexpr int PW = PagedRow<kD>::kWidth;
         const int j = lane & 7;
@@ -200,7 +202,7 @@ struct PagedSimt {
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float l = __shfl_sync(DA_FULL_MASK, st.l, keeper(lane, r));
+            const float m = __shfl_sync(DA_FULL_MASK, st.m, keeper(lane, r)), l = __shfl_sync(DA_FULL_MASK, st.l, keeper(lane, r));
             if (r >= rows || lane >= 8) continue;
             float *out = out_row<float>(p, item, r, kD, index);
 #pragma unroll
@@ -208,7 +210,7 @@ struct PagedSimt {
                 const float4 o = st.o[r][i];
                 if (has(j, i))
                     *reinterpret_cast<float4 *>(out + 4 * (j + 8 * i)) =
-                        l > 0.f ? make_float4(o.x / l, o.y / l, o.z / l, o.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        m == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
             }
         }
     }

@@ -134,6 +134,11 @@ struct PagedMma {
         return l + __shfl_xor_sync(DA_FULL_MASK, l, 2);
     }
 
+    __device__ __forceinline__ static void attended(State &st) {
+#pragma unroll
+        for (int half = 0; half < NR; ++half) st.m[half] = fmaxf(st.m[half], kLowest);
+    }
+
     __device__ __forceinline__ static void publish(State &st, float *dst, int lane, int rows) {
         constexpr int PW = PagedRow<kD>::kWidth;
         const int qd = lane & 3;
@@ -158,7 +163,7 @@ struct PagedMma {
             if (r >= rows) continue;
             size_t index;
             T *out = out_row<T>(p, item, r, kD, index);
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float inv = st.m[half] == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
             for (int d = 0; d < NT; ++d)
                 *reinterpret_cast<uint32_t *>(out + 8 * d + 2 * qd) =

@@ -169,8 +169,8 @@ class PagedKVCache:
         Logits are scaled by `scale` (default 1 / sqrt(D)).  Returns (n_sequences, Hq, D); with `return_lse` also the float32
         log-sum-exp of the scaled logits (n_sequences, Hq).  A sequence of length 0 gives zeros and -inf.  What pages hold beyond
         the attended tokens does not matter, NaN and infinities included; attended keys and values are taken to be finite.
-        The same inputs give the same bits.  Tokens in pages outside the pool are left out and lengths outside the
-        table are cut; `check_status` reports both."""
+        Where there are tokens, a row of q with a NaN or an infinity gives NaN, and no other row does.  The same inputs give the same
+        bits.  Tokens in pages outside the pool are left out and lengths outside the table are cut; `check_status` reports both."""
         n, columns, table_stride = self._check_table(page_table, lengths)
         q = self._check_heads(q, "q", n, None)
         hq = q.shape[1]

@@ -699,7 +699,7 @@ DA_API int da_append_pages(const da_append_pages_args *args);
  * order.  lengths is read on the device: a captured call follows it.
  *
  * q            (n_sequences, n_kv_heads * rep, head_dim), strides (sequence, head)
- * out          (n_sequences, n_kv_heads * rep, head_dim) contiguous; a sequence of length 0: zeros
+ * out          (n_sequences, n_kv_heads * rep, head_dim) contiguous; a sequence of length 0: zeros; a row of q that is not finite: NaN
  * lse          optional (n_sequences, n_kv_heads * rep) float32: log-sum-exp of the scaled scores, -inf for length 0
  * workspace    da_paged_attention_workspace_bytes() bytes, 16-byte aligned; holds nothing between calls, must not be shared by
  *              calls that may run at the same time
