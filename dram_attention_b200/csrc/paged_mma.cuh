@@ -10,6 +10,8 @@
 // (64 of 5000: 123, so 116), slower between them (60 of 3000, 8 heads of 80 and 96: 74 and 86 us, 79 and 93; 128 channels equal).
 #pragma once
 
+#include <type_traits>
+
 #include "mma_sync.cuh"
 #include "paged_attn.cuh"
 
@@ -26,6 +28,11 @@ struct PagedMma {
     static constexpr int ROWB = kD * 2, kTogether = paged_mma_together(kD), kStageBytes = paged_mma_stage(kD);
     static constexpr int KSTEPS = kD / 16, NT = kD / 8, NR = FULL ? 2 : 1;
     static constexpr int kScratch = 0;
+    // Weights, in (0, 1], and all that is summed with them are kept kWeight times as large: float16 has nothing between 0 and 2^-24, and
+    // many weights down there are a share of the sum (32 000 of 2.8e-8 beside one of 1: 0.0009, half a step is 0.0005).  So they are
+    // lost below 2^-40 of the largest; bfloat16 has the range of float32.  Scaling them takes 2 % of 256 channels and twelve rows (64 x
+    // 2000 tokens, 2 heads: 55.8 us, so 57.0), elsewhere less than the clock varies.
+    static constexpr float kWeight = std::is_same<T, __half>::value ? 32768.f : 1.f;
     __device__ __forceinline__ static constexpr int offset(int t) { return t * 2 * ROWB + t / kTogether * 16; }
     static_assert(kD % 16 == 0, "whole k-steps");
 
@@ -78,8 +85,9 @@ struct PagedMma {
             mma(ks & 1 ? t0 : s0, a, b[0], b[1]);
             mma(ks & 1 ? t1 : s1, a, b[2], b[3]);
         }
-        // The weights take part in the second product as the sum of two 16-bit numbers: rounded to one, they alone put bfloat16
-        // outputs 1.2 times as far from the 64-bit ones as their own rounding does, and memory hides the products.
+        // The weights take part in the second product as the sum of two 16-bit numbers, which leave 2^-16 of them in bfloat16 and
+        // 2^-22 in float16: rounded to one, they alone put bfloat16 outputs 1.2 times as far from the 64-bit ones as their own
+        // rounding does, and memory hides the products.
         uint32_t pa[NR][2], pb[NR][2];
 #pragma unroll
         for (int half = 0; half < NR; ++half) {
@@ -99,7 +107,7 @@ struct PagedMma {
             const float ms = m == -INFINITY ? 0.f : m;
             const float alpha = fast_exp2(st.m[half] - ms);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = fast_exp2(v[i] - ms);
+            for (int i = 0; i < 4; ++i) v[i] = fast_exp2(v[i] - ms) * kWeight;
             st.l[half] = st.l[half] * alpha + ((v[0] + v[1]) + (v[2] + v[3]));
             st.m[half] = m;
             if (__any_sync(DA_FULL_MASK, alpha != 1.f)) {   // once the maxima have settled there is nothing to rescale
@@ -144,12 +152,13 @@ struct PagedMma {
         const int qd = lane & 3;
 #pragma unroll
         for (int half = 0; half < NR; ++half) {
-            const float l = row_sum(st.l[half]);
+            const float l = row_sum(st.l[half]) * (1.f / kWeight);
             const int r = (lane >> 2) + 8 * half;
             if (r >= rows) continue;
 #pragma unroll
             for (int d = 0; d < NT; ++d)
-                *reinterpret_cast<float2 *>(dst + r * PW + 8 * d + 2 * qd) = make_float2(st.o[d][2 * half], st.o[d][2 * half + 1]);
+                *reinterpret_cast<float2 *>(dst + r * PW + 8 * d + 2 * qd) =
+                    make_float2(st.o[d][2 * half] * (1.f / kWeight), st.o[d][2 * half + 1] * (1.f / kWeight));
             if (qd == 0) *reinterpret_cast<float2 *>(dst + r * PW + kD) = make_float2(st.m[half], l);
         }
     }
@@ -168,7 +177,7 @@ struct PagedMma {
             for (int d = 0; d < NT; ++d)
                 *reinterpret_cast<uint32_t *>(out + 8 * d + 2 * qd) =
                     MmaTraits<T>::pack(st.o[d][2 * half] * inv, st.o[d][2 * half + 1] * inv);
-            if (qd == 0 && p.lse) p.lse[index] = natural_lse(st.m[half], l);
+            if (qd == 0 && p.lse) p.lse[index] = natural_lse(st.m[half], l * (1.f / kWeight));
         }
     }
 };

@@ -1,9 +1,16 @@
-"""GPU tests of attention over a paged cache: queries that are no numbers."""
+"""GPU tests of attention over a paged cache: queries that are no numbers, and how finely the weights are kept.
+
+Tolerance, in the terms of test_gpu_paged.py (u half a step of the element type, e what the logits and sums are off by, A the
+weighted mean of |v|).  In 16-bit types a weight takes part in the second product as the sum of two numbers of the type: the first
+leaves at most u of it, the second u of that, so u^2 relative.  Float16 has no numbers between 0 and 2^-24: what lies there is off by
+2^-25, and the weights are kept as multiples of 2^-15 of the largest, so a token by at most 2^-40 of the largest weight."""
+
+import math
 
 import pytest
 import torch
 
-from tests.test_gpu_paged import DEV, TYPES, _pool, _randn, da  # noqa: F401
+from tests.test_gpu_paged import DEV, HALF_STEP, TYPES, _pool, _randn, da  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +65,34 @@ def test_a_row_whose_pages_are_all_bad_gives_zeros_for_any_query(da, dtype):
     with pytest.raises(RuntimeError, match="page id"):
         cache.check_status()
     assert bool((out == 0).all()) and bool((lse == -float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rep", [4, 12])
+@pytest.mark.parametrize("n,batch", [(16, 1), (1000, 1), (1000, 2500), (32768, 2500)])
+def test_many_small_weights_beside_a_large_one(da, dtype, rep, n, batch):
+    """One key 17.4 above the others, whose values are 1 and its own 0: the output is the others' share.  Many sequences share the
+    pages, so that a warp has all of an item."""
+    d, page = 64, 16
+    pool = torch.zeros(1, -(-n // page), page, 2, d, dtype=dtype, device=DEV)
+    pool[0, :, :, 1] = 1.0
+    outlier = n // 2
+    pool[0, outlier // page, outlier % page, 0, 0] = 139.0
+    pool[0, outlier // page, outlier % page, 1] = 0.0
+    cache = da.PagedKVCache.over(pool)
+    q = torch.zeros(batch, rep, d, dtype=dtype, device=DEV)
+    q[..., 0] = 1.0
+    table = torch.arange(pool.shape[1], dtype=torch.int32, device=DEV).expand(batch, -1)
+    out, lse = cache.attend(q, table, torch.full((batch,), n, dtype=torch.int32, device=DEV), return_lse=True)
+    cache.check_status()
+    small = (n - 1) * math.exp(-139.0 / 8)
+    want = small / (1 + small)
+    u = HALF_STEP[dtype]
+    e = (d + 8) * 2.0 ** -23 * 139.0 / 8 + (n / 16 + 64) * 2.0 ** -23
+    tol = want * (2 * (e + (u * u if dtype != torch.float32 else 0.0)) + u) * (1 + u)
+    if dtype == torch.float16:
+        tol += n * 2.0 ** -40 + 2.0 ** -25
+    err = float((out.double() - want).abs().max())
+    assert err <= tol, (err, tol, want)
+    want_lse = 139.0 / 8 + math.log1p(small)
+    assert float((lse.double() - want_lse).abs().max()) <= e + 2.0 ** -22 * (1 + want_lse)
