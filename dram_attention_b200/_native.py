@@ -11,6 +11,7 @@ import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_longlong, c_size_t, c_void_p, POINTER
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdram_attention_b200.so")
@@ -192,6 +193,16 @@ def stream_ptr() -> int:
 
 def status_message(bits: int) -> str:
     return "; ".join(t for b, t in _STATUS_TEXT.items() if bits & b)
+
+
+def forward_mode() -> bool:
+    """Whether derivatives in forward mode are being taken."""
+    return forward_ad._current_level >= 0
+
+
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether one of them comes in by this tensor."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def require_cuda(t: torch.Tensor, name: str) -> None:

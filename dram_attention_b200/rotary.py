@@ -96,7 +96,7 @@ class Rotary:
     def __call__(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
         """q (s, Hq, D) or (b, s, Hq, D), k the same with its own number of heads; positions int32 or int64, (s,) or (b, s),
         magnitudes below 2^31.  Channels from rotary_dim on pass unchanged.  Returns the rotated pair (new tensors);
-        differentiable in q and k.  (As with every differentiable call: let go of results of eager calls on the same leaves
+        differentiable in q and k, backwards and in forward mode.  (As with every differentiable call: let go of results of eager calls on the same leaves
         before a call and its backward pass are captured into a graph, torch ties the leaves' gradients to the eager stream.)"""
         qs, ks, device = q.shape, k.shape, q.get_device()
         lead = len(qs) - 2
@@ -115,13 +115,18 @@ class Rotary:
         inv_freq = self._inv_freq
         assert k.get_device() == positions.get_device() == inv_freq.get_device() == device, \
             f"k ({k.device}), positions ({positions.device}) and inv_freq ({inv_freq.device}) must be on the device of q ({q.device})"
-        if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
+        if _derives(q) or _derives(k):
             return _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
         return _rotate(q, k, positions, inv_freq, self.factor, self.interleaved, False)
 
 
 _POSITION_TYPES = (torch.int32, torch.int64)
 _NOTHING = (0, 0, (0, 0, 0), 0)
+
+
+def _derives(t: torch.Tensor) -> bool:
+    """Whether something asks for the derivative by this tensor"""
+    return (t.requires_grad and torch.is_grad_enabled()) or _native.has_tangent(t)
 
 
 def _side(t: torch.Tensor):
@@ -152,12 +157,16 @@ def _rotate(q, k, positions, inv_freq, factor, interleaved, transposed):
 
 
 class _Rotate(torch.autograd.Function):
-    """The rotation is linear in q and k: its gradient is the transposed rotation, which is one again."""
+    """The rotation is linear in q and k: its gradient is the transposed rotation, which is one again, and in forward mode the
+    tangents are rotated like the heads."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, factor, interleaved, transposed):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (factor, interleaved, transposed)
+        if _native.forward_mode():
+            ctx.save_for_forward(positions, inv_freq)
+            ctx.shapes = (q.shape, k.shape)
         ctx.set_materialize_grads(False)
         return _rotate(q, k, positions, inv_freq, factor, interleaved, transposed)
 
@@ -169,12 +178,22 @@ class _Rotate(torch.autograd.Function):
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is None and dk is None:
             return (None,) * 7
-        how = (positions, inv_freq, factor, interleaved, not transposed)
-        if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in (dq, dk)):
-            # (a second derivative: a missing gradient is passed on as one without elements)
-            none = lambda g, like: like.new_empty(like.shape[:-2] + (0, like.shape[-1])) if g is None else g
-            q, k = _Rotate.apply(none(dq, dk), none(dk, dq), *how)
-            dq, dk = (None if dq is None else q), (None if dk is None else k)
-        else:
-            dq, dk = _rotate(dq, dk, *how)
-        return dq, dk, None, None, None, None, None
+        return _linear(dq, dk, positions, inv_freq, factor, interleaved, not transposed) + (None,) * 5
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        positions, inv_freq = ctx.saved_tensors
+        tangents = _linear(tq, tk, positions, inv_freq, *ctx.how)
+        # (torch wants a tangent for each output)
+        like = tq if tk is None else tk
+        return tuple(like.new_zeros(shape) if t is None else t for t, shape in zip(tangents, ctx.shapes))
+
+
+def _linear(x, y, *how):
+    """The rotation of what belongs to q and to k, gradients or tangents, one of which may be missing; itself differentiable"""
+    if (x is not None and _derives(x)) or (y is not None and _derives(y)):
+        # (a second derivative: what is missing is passed on as a tensor without elements)
+        none = lambda t, like: like.new_empty(like.shape[:-2] + (0, like.shape[-1])) if t is None else t
+        a, b = _Rotate.apply(none(x, y), none(y, x), *how)
+        return (None if x is None else a), (None if y is None else b)
+    return _rotate(x, y, *how)

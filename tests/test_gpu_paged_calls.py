@@ -1,0 +1,74 @@
+"""GPU tests of how the paged-cache operators are called: derivatives in forward mode, inputs that need none, reports of calls on
+other streams, the documented decode step."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tests.test_gpu_paged import DEV, _frequencies, _randn, da  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _rotation(da, **how):
+    return da.Rotary(_frequencies(64), factor=1.25, **how), torch.arange(5, device=DEV) * 1001
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_forward_mode_derivatives_of_the_rotation(da, dtype, interleaved):
+    """Linear in q and k: the tangents are rotated like the heads, bit by bit."""
+    r, p = _rotation(da, interleaved=interleaved)
+    q, k, tq, tk = (_randn(s, 5, h, 64, dtype=dtype) for s, h in ((1, 4), (2, 2), (3, 4), (4, 2)))
+    want, want_t = r(q, k, p), r(tq, tk, p)
+    apart = _randn(5, 5, 4, 128, dtype=dtype)[..., ::2]
+    for grad in (False, True):
+        with forward_ad.dual_level():
+            a, b = (x.clone().requires_grad_(grad) for x in (q, k))
+            both = r(forward_ad.make_dual(a, tq), forward_ad.make_dual(b, tk), p)
+            for got, x, t in zip(both, want, want_t):
+                primal, tangent = forward_ad.unpack_dual(got)
+                assert torch.equal(primal, x) and torch.equal(tangent, t)
+            # one side alone
+            one = r(forward_ad.make_dual(a, tq), b, p)
+            assert torch.equal(forward_ad.unpack_dual(one[0]).tangent, want_t[0])
+            rest = forward_ad.unpack_dual(one[1]).tangent
+            assert rest is None or bool((rest == 0).all())
+            other = r(a, forward_ad.make_dual(b, tk), p)
+            assert torch.equal(forward_ad.unpack_dual(other[1]).tangent, want_t[1]) and torch.equal(other[0].detach(), want[0])
+            # tangents with gaps between their channels, and under no_grad
+            with torch.no_grad():
+                strided = r(forward_ad.make_dual(a.detach(), apart), b.detach(), p)[0]
+            assert torch.equal(forward_ad.unpack_dual(strided).tangent, r(apart, k, p)[0])
+
+
+def test_forward_mode_through_the_gradient_and_back(da):
+    """Forward over reverse and reverse over forward: with y = R q and a loss of |y|^2 / 2 the gradient is f^2 q, its derivative
+    along t is f^2 t; the sum of R t against w has R^T w as its gradient in t."""
+    r, p = _rotation(da)
+    q, k, t, w = _randn(1, 5, 4, 64), _randn(2, 5, 2, 64), _randn(3, 5, 4, 64), _randn(4, 5, 4, 64)
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(q.clone().requires_grad_(), t)
+        y, _ = r(x, k, p)
+        (g,) = torch.autograd.grad((y * y).sum() / 2, x)
+        got = forward_ad.unpack_dual(g).tangent
+        # two rotations, each off by at most 8 * 2^-24 of the sum of the pair's magnitudes times the factor
+        size = (t.unflatten(-1, (32, 2)).abs().sum(-1, keepdim=True).expand(-1, -1, -1, 2).flatten(-2)).double()
+        assert bool(((got.double() - 1.5625 * t.double()).abs() <= 2 * 16 * 2.0 ** -24 * 1.5625 * size).all())
+    with forward_ad.dual_level():
+        s = t.clone().requires_grad_()
+        y, _ = r(forward_ad.make_dual(q, s), k, p)
+        (g,) = torch.autograd.grad((forward_ad.unpack_dual(y).tangent * w).sum(), s)
+    a = q.clone().requires_grad_()
+    (want,) = torch.autograd.grad((r(a, k, p)[0] * w).sum(), a)
+    assert torch.equal(g, want)
+
+
+def test_function_transforms_are_refused(da):
+    """What the rotation has no rule for ends in an error, never in a derivative of zero."""
+    r, p = _rotation(da)
+    q, k = _randn(1, 5, 4, 64), _randn(2, 5, 2, 64)
+    for call in (lambda: torch.func.jvp(lambda x: r(x, k, p)[0], (q,), (q,)), lambda: torch.func.grad(lambda x: r(x, k, p)[0].sum())(q),
+                 lambda: torch.func.vmap(lambda x: r(x, k, p)[0])(q[None])):
+        with pytest.raises(Exception):
+            call()
