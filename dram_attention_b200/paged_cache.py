@@ -89,6 +89,7 @@ class PagedKVCache:
         assert t.dtype is self._dtype, f"{name} must be {self._dtype} like the pages, got {t.dtype}"
         assert not (t.requires_grad and torch.is_grad_enabled()), \
             f"{name} requires a gradient, which the paged cache does not pass on: detach it or call under torch.no_grad()"
+        assert not _native.has_tangent(t), f"{name} has a tangent, which the paged cache does not pass on: detach it"
         return t if t.stride(2) == 1 else t.contiguous()
 
     def _wrong_device(self, t: torch.Tensor, name: str) -> None:

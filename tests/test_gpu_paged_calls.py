@@ -72,3 +72,22 @@ def test_function_transforms_are_refused(da):
                  lambda: torch.func.vmap(lambda x: r(x, k, p)[0])(q[None])):
         with pytest.raises(Exception):
             call()
+
+
+def test_tangents_are_refused_where_nothing_passes_them_on(da):
+    cache = da.PagedKVCache(4, 16, 2, 64)
+    table, n = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    k, q = _randn(1, 1, 2, 64, dtype=torch.bfloat16), _randn(2, 1, 4, 64, dtype=torch.bfloat16)
+    r = da.Rotary(_frequencies(64))
+    with forward_ad.dual_level():
+        dk, dq = forward_ad.make_dual(k, k), forward_ad.make_dual(q, q)
+        for bad in (lambda: cache.append_(dk, k, table, n), lambda: cache.append_(k, dk, table, n),
+                    lambda: cache.append_(k, k, table, n, q=dq, rotary=r), lambda: cache.attend(dq, table, n)):
+            with pytest.raises(AssertionError, match="tangent"):
+                bad()
+            with torch.no_grad(), pytest.raises(AssertionError, match="tangent"):
+                bad()
+        assert bool((cache.pages == 0).all())
+        cache.append_(k, k, table, n)
+        cache.attend(q, table, n)
+    cache.check_status()
