@@ -96,8 +96,9 @@ class Rotary:
     def __call__(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
         """q (s, Hq, D) or (b, s, Hq, D), k the same with its own number of heads; positions int32 or int64, (s,) or (b, s),
         magnitudes below 2^31.  Channels from rotary_dim on pass unchanged.  Returns the rotated pair (new tensors);
-        differentiable in q and k, backwards and in forward mode.  (As with every differentiable call: let go of results of eager calls on the same leaves
-        before a call and its backward pass are captured into a graph, torch ties the leaves' gradients to the eager stream.)"""
+        differentiable in q and k, backwards and in forward mode; the output of one that needs no derivative needs none.  (As
+        with every differentiable call: let go of results of eager calls on the same leaves before a call and its backward pass are
+        captured into a graph, torch ties the leaves' gradients to the eager stream.)"""
         qs, ks, device = q.shape, k.shape, q.get_device()
         lead = len(qs) - 2
         assert 1 <= lead <= 2 and len(ks) == lead + 2 and ks[0] == qs[0] and ks[lead - 1] == qs[lead - 1] and ks[-1] == qs[-1], \
@@ -115,8 +116,11 @@ class Rotary:
         inv_freq = self._inv_freq
         assert k.get_device() == positions.get_device() == inv_freq.get_device() == device, \
             f"k ({k.device}), positions ({positions.device}) and inv_freq ({inv_freq.device}) must be on the device of q ({q.device})"
-        if _derives(q) or _derives(k):
-            return _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
+        by_q, by_k = _derives(q), _derives(k)
+        if by_q or by_k:
+            q2, k2 = _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
+            # (the function gives both outputs a place in the graph)
+            return q2 if by_q else q2.detach(), k2 if by_k else k2.detach()
         return _rotate(q, k, positions, inv_freq, self.factor, self.interleaved, False)
 
 

@@ -91,3 +91,17 @@ def test_tangents_are_refused_where_nothing_passes_them_on(da):
         cache.append_(k, k, table, n)
         cache.attend(q, table, n)
     cache.check_status()
+
+
+def test_an_input_that_needs_no_gradient_has_an_output_that_needs_none(da):
+    """Frozen keys beside trained queries: their rotation can be appended to a cache like any other."""
+    r, p = _rotation(da)
+    q, k = _randn(1, 5, 4, 64).requires_grad_(), _randn(2, 5, 2, 64)
+    q2, k2 = r(q, k, p)
+    assert q2.requires_grad and not k2.requires_grad
+    cache = da.PagedKVCache(1, 16, 2, 64, dtype=torch.float32)
+    starts = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    cache.append_(k2, k, torch.zeros(1, 1, dtype=torch.int32, device=DEV), starts[1:], starts=starts)
+    assert torch.equal(cache.pages[:, 0, :5, 0].transpose(0, 1), r(q, k, p)[1])
+    q2, k2 = r(q.detach(), k.requires_grad_(), p)
+    assert k2.requires_grad and not q2.requires_grad
