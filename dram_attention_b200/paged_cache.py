@@ -208,10 +208,13 @@ class PagedKVCache:
         return entry
 
     def check_status(self) -> None:
-        """Synchronises; raises if any call on this pool flagged a problem since the last check."""
+        """Waits for all streams of the device; raises if any call on this pool flagged a problem since the last check.  (Calls that
+        other threads enqueue meanwhile may be reported here or be missed.)"""
+        torch.cuda.synchronize(self._device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            torch.cuda.synchronize(self._device)   # (or a later call on another stream could flag a problem first)
             raise RuntimeError("dram_attention_b200 device status: " + "; ".join(t for b, t in _STATUS_TEXT.items() if bits & b))
 
 

@@ -105,3 +105,29 @@ def test_an_input_that_needs_no_gradient_has_an_output_that_needs_none(da):
     assert torch.equal(cache.pages[:, 0, :5, 0].transpose(0, 1), r(q, k, p)[1])
     q2, k2 = r(q.detach(), k.requires_grad_(), p)
     assert k2.requires_grad and not q2.requires_grad
+
+
+def test_status_of_calls_on_other_streams(da):
+    cache = da.PagedKVCache(4, 16, 2, 64)
+    bad, n = torch.full((1, 1), 9, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    q = torch.ones(1, 4, 64, dtype=torch.bfloat16, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)            # (some 50 ms: the call has not run when its report is asked for)
+            cache.attend(q, bad, n)
+        with pytest.raises(RuntimeError, match="page id"):
+            cache.check_status()
+    cache.check_status()
+    # asked for on a busy stream, reported on another: nothing that comes after the report is erased by it
+    with torch.cuda.stream(side):
+        cache.attend(q, bad, n)
+    with pytest.raises(RuntimeError, match="page id"):
+        cache.check_status()
+    with torch.cuda.stream(side):
+        cache.attend(q, bad, n)
+    side.synchronize()
+    with pytest.raises(RuntimeError, match="page id"):
+        cache.check_status()
+    cache.check_status()
