@@ -131,3 +131,33 @@ def test_status_of_calls_on_other_streams(da):
     with pytest.raises(RuntimeError, match="page id"):
         cache.check_status()
     cache.check_status()
+
+
+def test_documented_decode_step_leaves_rows_alone_that_are_not_in_use(da):
+    """lengths.add_(lengths.sign()): rows of length 0 stay so, whatever their table holds; one joins by its prompt."""
+    cache = da.PagedKVCache(8, 16, 2, 64)
+    r = da.Rotary(_frequencies(64))
+    table = torch.tensor([[0, 1], [1, 0], [-1, -1], [2, 3]], dtype=torch.int32, device=DEV)     # rows 1 and 2 are free, 1 with an old entry
+    lengths = torch.zeros(4, dtype=torch.int32, device=DEV)
+    prompt = _randn(1, 25, 2, 64, dtype=torch.bfloat16)
+    lengths[0], lengths[3] = 20, 5
+    cache.append_(prompt, prompt, table, lengths, starts=torch.tensor([0, 20, 20, 20, 25], dtype=torch.int32, device=DEV), rotary=r)
+    k, q = _randn(2, 4, 2, 64, dtype=torch.bfloat16), _randn(3, 4, 4, 64, dtype=torch.bfloat16)
+
+    def step():
+        lengths.add_(lengths.sign())
+        return cache.attend(cache.append_(k, k, table, lengths, q=q, rotary=r), table, lengths)
+
+    kept = cache.pages.clone()
+    out = step()
+    cache.check_status()
+    assert lengths.tolist() == [21, 0, 0, 6] and bool((out[1:3] == 0).all()) and bool((out[0] != 0).any())
+    assert (cache.pages != kept).flatten(3).any(-1).any(0).nonzero().tolist() == [[1, 4], [2, 5]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    table[1], lengths[1] = torch.tensor([4, 5], dtype=torch.int32, device=DEV), 3
+    cache.append_(prompt[:3], prompt[:3], table[1:2], lengths[1:2], starts=torch.tensor([0, 3], dtype=torch.int32, device=DEV), rotary=r)
+    graph.replay()
+    cache.check_status()
+    assert lengths.tolist() == [22, 4, 0, 7]
