@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_paged import DEV, HALF_STEP, TYPES, _pool, _randn, da  # noqa: F401
+from tests.test_gpu_paged import DEV, HALF_STEP, TYPES, _assert_attended, _attention, _pool, _randn, da  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,41 @@ def test_many_small_weights_beside_a_large_one(da, dtype, rep, n, batch):
     assert err <= tol, (err, tol, want)
     want_lse = 139.0 / 8 + math.log1p(small)
     assert float((lse.double() - want_lse).abs().max()) <= e + 2.0 ** -22 * (1 + want_lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,rep", [(64, 3), (64, 16), (80, 5), (128, 4), (256, 12)])
+def test_weights_are_kept_to_twice_the_bits_of_the_type(da, dtype, d, rep):
+    """Few tokens, so that the values of a row cancel in many channels and their outputs show the weights' own errors: rounded once to
+    bfloat16 or float16 they would leave the bound."""
+    lengths = [2 + i % 19 for i in range(200)]
+    pool, table, keys, values = _pool(64, lengths, 1, 16, d, dtype)
+    q = _randn(65, len(lengths), rep, d, dtype=dtype)
+    cache = da.PagedKVCache.over(pool)
+    out = cache.attend(q, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.25 * d ** -0.5)
+    want, _, tol, rounded_once = _fine_tolerance(q, keys, values, 0.25 * d ** -0.5)
+    _assert_attended(out, want, tol)
+    if dtype != torch.float32:       # (the bound tells the two apart: the definition with weights of one number is outside it)
+        assert bool(((rounded_once - want).abs() > tol).any())
+
+
+def _fine_tolerance(q, keys, values, scale):
+    """(out, lse, tolerance of out, out with every weight rounded once) in 64 bits"""
+    out, lse, _, _ = _attention(q, keys, values, 0, scale)
+    u = HALF_STEP[q.dtype]
+    u_w = 0.0 if q.dtype == torch.float32 else u * u
+    tol, once = torch.zeros_like(out), torch.zeros_like(out)
+    for b, (k, v) in enumerate(zip(keys, values)):
+        hk, n, d = k.shape
+        x = q[b].double().reshape(hk, -1, d)
+        s = x @ k.transpose(1, 2) * scale
+        size = (x.abs() @ k.abs().transpose(1, 2)).amax(-1) * abs(scale)
+        w = torch.softmax(s, -1)
+        mean = w @ v.abs()
+        e = (d + 8) * 2.0 ** -23 * size + (n / 16 + 64) * 2.0 ** -23
+        tol[b] = (mean * (u_w + 2 * e)[..., None] * (1 + u) + u * (w @ v).abs()).reshape(out[b].shape)
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        once[b] = ((p.to(q.dtype).double() @ v) / p.sum(-1, keepdim=True)).to(q.dtype).double().reshape(out[b].shape)
+    if q.dtype == torch.float16:
+        tol += 2.0 ** -25 + 20 * 2.0 ** -40 * max(float(v.abs().max()) for v in values)
+    return out, lse, tol, once
