@@ -21,7 +21,12 @@ constexpr int paged_mma_together(int head_dim) { return head_dim == 64 || head_d
 constexpr int paged_mma_stage(int head_dim) { return kPagedUnit * 4 * head_dim + kPagedUnit / paged_mma_together(head_dim) * 16; }
 
 // FULL: up to 16 query rows; otherwise up to 8 (rows 8..15 of the tile are zero and nothing is kept of them).
-template <typename T, int D_, bool FULL>
+// LONG: a warp may have more than kPagedRun units of one item.  The tensor cores cut off the low bits of the sums that they add to,
+// always towards zero, so an accumulator that they keep loses up to 2^-23 of itself with every product: float16 outputs of equal
+// weights and values near 1 are 1e-4 too small on average for 131 072 tokens in one warp and 4e-3 for a million, against half a step
+// of 5e-4.  A LONG unit's product is made alone and added in float32, rounded to nearest (1e-6).  Batches that need none of it would
+// take 3 % longer by it with 64 channels, 8 % with 256 (registers spill: 64 x 2000 tokens 53.3 us, 58.1), the same with 96 and 128.
+template <typename T, int D_, bool FULL, bool LONG>
 struct PagedMma {
     using Elem = T;
     static constexpr int kD = D_, kRows = FULL ? 16 : 8;
@@ -39,7 +44,7 @@ struct PagedMma {
     struct State {
         uint32_t q[NR][2][KSTEPS];    // A fragments: [row half][k half][k-step]
         float m[NR], l[NR];           // row maximum (the same in the four lanes of a row), this lane's share of the weight sum
-        float o[NT][4];
+        float o[NT][4];               // (rows 8..15: of no meaning unless FULL)
     };
 
     __device__ __forceinline__ static void begin(State &st, const PagedParams &p, int b, int head, int group, int rows, int lane, unsigned char *) {
@@ -67,6 +72,11 @@ struct PagedMma {
         else MmaTraits<T>::mma(d, a[0][0], a[0][1], b0, b1);
     }
 
+    __device__ __forceinline__ static void product(float (&d)[4], const uint32_t (&a)[NR][2], uint32_t b0, uint32_t b1) {
+        if constexpr (FULL) MmaTraits<T>::product(d, a[0][0], a[1][0], a[0][1], a[1][1], b0, b1);
+        else MmaTraits<T>::product(d, a[0][0], 0u, a[0][1], 0u, b0, b1);
+    }
+
     __device__ __forceinline__ static void consume(State &st, const unsigned char *unit, uint32_t mask, int lane, float scale_log2) {
         const int qd = lane & 3, tile = lane >> 3, tr = lane & 7;
         // key tiles of a k-step: tokens 0..7 and 8..15, channels 0..7 and 8..15 of it
@@ -89,6 +99,7 @@ struct PagedMma {
         // 2^-22 in float16: rounded to one, they alone put bfloat16 outputs 1.2 times as far from the 64-bit ones as their own
         // rounding does, and memory hides the products.
         uint32_t pa[NR][2], pb[NR][2];
+        float alpha[NR];
 #pragma unroll
         for (int half = 0; half < NR; ++half) {
             // this lane: row lane / 4 + 8 * half, tokens 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
@@ -105,16 +116,16 @@ struct PagedMma {
             mx = fmaxf(mx, __shfl_xor_sync(DA_FULL_MASK, mx, 2));
             const float m = fmaxf(st.m[half], mx);
             const float ms = m == -INFINITY ? 0.f : m;
-            const float alpha = fast_exp2(st.m[half] - ms);
+            alpha[half] = fast_exp2(st.m[half] - ms);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = fast_exp2(v[i] - ms) * kWeight;
-            st.l[half] = st.l[half] * alpha + ((v[0] + v[1]) + (v[2] + v[3]));
+            st.l[half] = st.l[half] * alpha[half] + ((v[0] + v[1]) + (v[2] + v[3]));
             st.m[half] = m;
-            if (__any_sync(DA_FULL_MASK, alpha != 1.f)) {   // once the maxima have settled there is nothing to rescale
+            if (!LONG && __any_sync(DA_FULL_MASK, alpha[half] != 1.f)) {   // once the maxima have settled there is nothing to rescale
 #pragma unroll
                 for (int d = 0; d < NT; ++d) {
-                    st.o[d][2 * half] *= alpha;
-                    st.o[d][2 * half + 1] *= alpha;
+                    st.o[d][2 * half] *= alpha[half];
+                    st.o[d][2 * half + 1] *= alpha[half];
                 }
             }
             pa[half][0] = MmaTraits<T>::pack(v[0], v[1]);
@@ -130,10 +141,22 @@ struct PagedMma {
         for (int d = 0; d < NT / 2; ++d) {
             uint32_t b[4];
             ldmatrix_x4_trans(b, values + d * 32);
-            mma(st.o[2 * d], pa, b[0], b[1]);
-            mma(st.o[2 * d + 1], pa, b[2], b[3]);
-            mma(st.o[2 * d], pb, b[0], b[1]);
-            mma(st.o[2 * d + 1], pb, b[2], b[3]);
+            if constexpr (!LONG) {
+                mma(st.o[2 * d], pa, b[0], b[1]);
+                mma(st.o[2 * d + 1], pa, b[2], b[3]);
+                mma(st.o[2 * d], pb, b[0], b[1]);
+                mma(st.o[2 * d + 1], pb, b[2], b[3]);
+            } else {
+                float x[2][4];
+                product(x[0], pa, b[0], b[1]);
+                product(x[1], pa, b[2], b[3]);
+                mma(x[0], pb, b[0], b[1]);
+                mma(x[1], pb, b[2], b[3]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2 * NR; ++i) st.o[2 * d + t][i] = fmaf(st.o[2 * d + t][i], alpha[i / 2], x[t][i]);
+            }
         }
     }
 
@@ -194,10 +217,18 @@ template <int D> struct PagedMmaShape {
     static_assert(kStages >= 2, "");
 };
 
+// Whether a warp's stretch can hold more than kPagedRun units (65 536 tokens) of an item, by what the tables have room for.
+constexpr long long kPagedRun = 4096;
+static bool paged_long_runs(const PagedParams &p, int warps) {
+    const long long room = p.window > 0 && p.window < p.capacity ? p.window : p.capacity, units = room / kPagedUnit + 2;
+    return units > kPagedRun && units * p.n_sequences * p.n_kv_heads * p.groups > kPagedRun * kPagedCtas * warps;
+}
+
 template <typename T, int D, bool FULL>
 static cudaError_t launch_paged_mma(const PagedParams &p, cudaStream_t stream) {
     using Shape = PagedMmaShape<D>;
-    return launch_paged<PagedMma<T, D, FULL>, Shape::kWarps, Shape::kStages>(p, stream);
+    if (paged_long_runs(p, Shape::kWarps)) return launch_paged<PagedMma<T, D, FULL, true>, Shape::kWarps, Shape::kStages>(p, stream);
+    return launch_paged<PagedMma<T, D, FULL, false>, Shape::kWarps, Shape::kStages>(p, stream);
 }
 
 template <typename T>

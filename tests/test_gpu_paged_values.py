@@ -134,3 +134,25 @@ def _fine_tolerance(q, keys, values, scale):
     if q.dtype == torch.float16:
         tol += 2.0 ** -25 + 20 * 2.0 ** -40 * max(float(v.abs().max()) for v in values)
     return out, lse, tol, once
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,rep,batch,n", [(64, 4, 1800, 1048576), (128, 12, 1200, 262144), (256, 2, 900, 196608), (96, 5, 1800, 196608)])
+def test_sums_over_very_many_tokens_in_one_warp(da, dtype, d, rep, batch, n):
+    """Equal weights over values near 1: the output is their mean.  The sequences share the pages, and there are as many as warps, so
+    that a warp has (nearly) all tokens of one.  Tolerance: the products of a unit and the join 64 * 2^-23; one rounding to nearest
+    per 16 tokens, 2^-24 of the sum each, which add up like independent ones, six deviations: 6 sqrt(n / 16) 2^-24; u of the output."""
+    if dtype == torch.float32:
+        batch, n = batch // 4, n // 4
+    pool = torch.zeros(1, n // 16, 16, 2, d, dtype=dtype, device=DEV)
+    pool[0, :, :, 1] = (1 + 0.25 * torch.rand(n // 16, 16, d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(66))).to(dtype)
+    table = torch.arange(n // 16, dtype=torch.int32, device=DEV).expand(batch, -1)
+    cache = da.PagedKVCache.over(pool)
+    out, lse = cache.attend(torch.zeros(batch, rep, d, dtype=dtype, device=DEV), table, torch.full((batch,), n, dtype=torch.int32, device=DEV),
+                            return_lse=True)
+    cache.check_status()
+    want = pool[0, :, :, 1].double().mean((0, 1))
+    tol = want * (64 * 2.0 ** -23 + 6 * math.sqrt(n / 16) * 2.0 ** -24 + HALF_STEP[dtype])
+    err = (out.double() - want).abs()
+    assert bool((err <= tol).all()), float((err / want).max())
+    assert float((lse.double() - math.log(n)).abs().max()) <= 2.0 ** -20 * (1 + math.log(n))
