@@ -41,7 +41,7 @@ class PagedKVCache:
     def over(cls, pages: torch.Tensor) -> "PagedKVCache":
         """The operators on a pool that exists already: (n_kv_heads, n_pages, page_size, 2, head_dim), pages of a head and
         heads at any distance (a multiple of 16 bytes), or the slot table of an LRU cache,
-        `lru.hbm_kv_cache.view(lru.num_kv_heads, -1, lru.page_size, 2, lru.head_dim)`."""
+        `lru.hbm_kv_cache.view(lru.num_kv_heads, -1, lru.page_size, 2, lru.head_dim)`.  Derivatives do not reach it."""
         self = cls.__new__(cls)
         self._set_pages(pages)
         return self
