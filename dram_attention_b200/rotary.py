@@ -134,21 +134,22 @@ def _derives(t: torch.Tensor) -> bool:
 
 
 def _side(t: torch.Tensor):
-    """The output for q or k and what the call is told of the pair: addresses, strides (batch, token, head), heads"""
+    """The input (a copy where its channels lie apart: the caller keeps it until the call is enqueued, or its memory is another's), the
+    output, and what the call is told of the pair: addresses, strides (batch, token, head), heads"""
     strides = t.stride()
     if strides[-1] != 1:
         t = t.contiguous()
         strides = t.stride()
     out = torch.empty_like(t, memory_format=torch.contiguous_format)
     # (a tensor without elements takes part in the call no more than None does: its address is null)
-    return out, (t.data_ptr(), out.data_ptr(), strides[:3] if len(strides) == 4 else (0, strides[0], strides[1]), t.shape[-2])
+    return t, out, (t.data_ptr(), out.data_ptr(), strides[:3] if len(strides) == 4 else (0, strides[0], strides[1]), t.shape[-2])
 
 
 def _rotate(q, k, positions, inv_freq, factor, interleaved, transposed):
     """Enqueue da_rotate; q or k may be None.  Returns new tensors."""
     x = k if q is None else q
-    q2, (qp, qo, qs, hq) = (None, _NOTHING) if q is None else _side(q)
-    k2, (kp, ko, ks, hk) = (None, _NOTHING) if k is None else _side(k)
+    q, q2, (qp, qo, qs, hq) = (None, None, _NOTHING) if q is None else _side(q)
+    k, k2, (kp, ko, ks, hk) = (None, None, _NOTHING) if k is None else _side(k)
     if not qo and not ko:
         return q2, k2
     shape, device, ps = x.shape, x.get_device(), positions.stride()

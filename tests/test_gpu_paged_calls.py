@@ -161,3 +161,22 @@ def test_documented_decode_step_leaves_rows_alone_that_are_not_in_use(da):
     graph.replay()
     cache.check_status()
     assert lengths.tolist() == [22, 4, 0, 7]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens", [5, 3000])
+def test_queries_and_keys_that_are_both_copied_for_the_call(da, dtype, tokens):
+    """Channels at a distance: the copies of q and k live side by side until the rotation is enqueued, forwards and backwards."""
+    r, p = da.Rotary(_frequencies(64)), torch.arange(tokens, device=DEV)
+    apart = lambda seed: _randn(seed, tokens, 4, 128, dtype=dtype)[..., ::2]
+    q, k, dq, dk = (apart(s) for s in range(1, 5))
+    dense = [x.contiguous() for x in (q, k, dq, dk)]
+    want, want_g = r(dense[0], dense[1], p), r(dense[2], dense[3], -p)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(r(q, k, p), want))
+        assert all(torch.equal(a, b) for a, b in zip(r(q, dense[1], p), want)) and all(torch.equal(a, b) for a, b in zip(r(dense[0], k, p), want))
+    x, y = dense[0].clone().requires_grad_(), dense[1].clone().requires_grad_()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(r(x, y, p), (x, y), (dq, dk)), want_g))
+    # gradients that are one number for every element
+    ones = torch.autograd.grad(r(x, y, p), (x, y), (torch.ones((), dtype=dtype, device=DEV).expand(x.shape), torch.zeros((), dtype=dtype, device=DEV).expand(y.shape)))
+    assert torch.equal(ones[0], r(torch.ones_like(x), y, -p)[0].detach()) and bool((ones[1] == 0).all())
