@@ -195,13 +195,8 @@ def status_message(bits: int) -> str:
     return "; ".join(t for b, t in _STATUS_TEXT.items() if bits & b)
 
 
-def forward_mode() -> bool:
-    """Whether derivatives in forward mode are being taken."""
-    return forward_ad._current_level >= 0
-
-
 def has_tangent(t: torch.Tensor) -> bool:
-    """Whether one of them comes in by this tensor."""
+    """Whether a derivative in forward mode is under way that comes in by this tensor."""
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 

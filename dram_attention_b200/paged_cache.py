@@ -8,6 +8,7 @@ import operator
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .rotary import Rotary
@@ -55,6 +56,7 @@ class PagedKVCache:
         _native.require_cuda(pages, "pages")
         assert all(size == 1 or stride == want for size, stride, want in zip(pages.shape[2:], pages.stride()[2:], (2 * d, d, 1))), \
             "the tokens of a page must be contiguous"
+        assert not pages.is_neg(), "pages must be plain memory, not the negative of another tensor's"
         piece = 16 // pages.element_size()
         assert pages.data_ptr() % 16 == 0 and all(s % piece == 0 for n, s in zip(pages.shape, pages.stride()[:2]) if n > 1), \
             "pages must start on 16-byte boundaries"
@@ -87,10 +89,11 @@ class PagedKVCache:
         if t.get_device() != self._device:
             self._wrong_device(t, name)
         assert t.dtype is self._dtype, f"{name} must be {self._dtype} like the pages, got {t.dtype}"
-        assert not (t.requires_grad and torch.is_grad_enabled()), \
-            f"{name} requires a gradient, which the paged cache does not pass on: detach it or call under torch.no_grad()"
-        assert not _native.has_tangent(t), f"{name} has a tangent, which the paged cache does not pass on: detach it"
-        return t if t.stride(2) == 1 else t.contiguous()
+        if t.requires_grad or forward_ad._current_level >= 0:
+            assert not (t.requires_grad and torch.is_grad_enabled()), \
+                f"{name} requires a gradient, which the paged cache does not pass on: detach it or call under torch.no_grad()"
+            assert not _native.has_tangent(t), f"{name} has a tangent, which the paged cache does not pass on: detach it"
+        return t if t.stride(2) == 1 and not t.is_neg() else t.resolve_neg().contiguous()
 
     def _wrong_device(self, t: torch.Tensor, name: str) -> None:
         _native.require_cuda(t, name)

@@ -8,6 +8,7 @@ import math
 from typing import Mapping, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -80,7 +81,7 @@ class Rotary:
         assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.numel() > 0, \
             f"inv_freq must be a float32 vector, got {tuple(inv_freq.shape)} {inv_freq.dtype}"
         _native.lib()
-        self._inv_freq = inv_freq.detach().contiguous()
+        self._inv_freq = inv_freq.detach().resolve_neg().contiguous()
         self._rotary_dim = 2 * inv_freq.numel()
         self.factor = float(factor)
         self.interleaved = bool(interleaved)
@@ -116,11 +117,12 @@ class Rotary:
         inv_freq = self._inv_freq
         assert k.get_device() == positions.get_device() == inv_freq.get_device() == device, \
             f"k ({k.device}), positions ({positions.device}) and inv_freq ({inv_freq.device}) must be on the device of q ({q.device})"
-        by_q, by_k = _derives(q), _derives(k)
-        if by_q or by_k:
-            q2, k2 = _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
-            # (the function gives both outputs a place in the graph)
-            return q2 if by_q else q2.detach(), k2 if by_k else k2.detach()
+        if q.requires_grad or k.requires_grad or forward_ad._current_level >= 0:
+            by_q, by_k = _derives(q), _derives(k)
+            if by_q or by_k:
+                q2, k2 = _Rotate.apply(q, k, positions, inv_freq, self.factor, self.interleaved, False)
+                # (the function gives both outputs a place in the graph)
+                return q2 if by_q else q2.detach(), k2 if by_k else k2.detach()
         return _rotate(q, k, positions, inv_freq, self.factor, self.interleaved, False)
 
 
@@ -134,11 +136,11 @@ def _derives(t: torch.Tensor) -> bool:
 
 
 def _side(t: torch.Tensor):
-    """The input (a copy where its channels lie apart: the caller keeps it until the call is enqueued, or its memory is another's), the
-    output, and what the call is told of the pair: addresses, strides (batch, token, head), heads"""
+    """The input (a copy where its channels lie apart or torch counts its memory as negated: the caller keeps it until the call is
+    enqueued, or its memory is another's), the output, and what the call is told of the pair: addresses, strides (batch, token, head), heads"""
     strides = t.stride()
-    if strides[-1] != 1:
-        t = t.contiguous()
+    if strides[-1] != 1 or t.is_neg():
+        t = t.resolve_neg().contiguous()
         strides = t.stride()
     out = torch.empty_like(t, memory_format=torch.contiguous_format)
     # (a tensor without elements takes part in the call no more than None does: its address is null)
@@ -169,7 +171,7 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, q, k, positions, inv_freq, factor, interleaved, transposed):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = (factor, interleaved, transposed)
-        if _native.forward_mode():
+        if forward_ad._current_level >= 0:
             ctx.save_for_forward(positions, inv_freq)
             ctx.shapes = (q.shape, k.shape)
         ctx.set_materialize_grads(False)
@@ -188,8 +190,9 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def jvp(ctx, tq, tk, *_):
         positions, inv_freq = ctx.saved_tensors
+        # (torch has a kind of zeros without memory, and wants a tangent for each output)
+        tq, tk = (t.clone() if t is not None and t._is_zerotensor() else t for t in (tq, tk))
         tangents = _linear(tq, tk, positions, inv_freq, *ctx.how)
-        # (torch wants a tangent for each output)
         like = tq if tk is None else tk
         return tuple(like.new_zeros(shape) if t is None else t for t, shape in zip(tangents, ctx.shapes))
 

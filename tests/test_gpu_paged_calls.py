@@ -180,3 +180,38 @@ def test_queries_and_keys_that_are_both_copied_for_the_call(da, dtype, tokens):
     # gradients that are one number for every element
     ones = torch.autograd.grad(r(x, y, p), (x, y), (torch.ones((), dtype=dtype, device=DEV).expand(x.shape), torch.zeros((), dtype=dtype, device=DEV).expand(y.shape)))
     assert torch.equal(ones[0], r(torch.ones_like(x), y, -p)[0].detach()) and bool((ones[1] == 0).all())
+
+
+def test_heads_and_gradients_that_are_negated_lazily(da):
+    """Imaginary parts of conjugates share memory with what they are the negative of; gradients arrive in that form too."""
+    r, p = _rotation(da)
+    real = lambda seed, *shape: _randn(seed, *shape)
+    zq, zk = torch.complex(real(1, 5, 4, 64), real(2, 5, 4, 64)), torch.complex(real(3, 5, 2, 64), real(4, 5, 2, 64))
+    apart = lambda z: z.conj().imag                                       # every second word
+    dense = lambda x: torch._neg_view(x)
+    for q, k in ((apart(zq), apart(zk)), (dense(zq.imag.contiguous()), dense(zk.imag.contiguous()))):
+        assert q.is_neg() and k.is_neg()
+        for a, b in zip(r(q, k, p), r(-zq.imag, -zk.imag, p)):
+            assert torch.equal(a, b)
+    q, k = zq.real.contiguous().requires_grad_(), zk.real.contiguous().requires_grad_()
+    dq, dk = dense(real(5, 5, 4, 64)), dense(real(6, 5, 2, 64))
+    got = torch.autograd.grad(r(q, k, p), (q, k), (dq, dk))
+    want = torch.autograd.grad(r(q, k, p), (q, k), (dq.resolve_neg(), dk.resolve_neg()))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # as it comes about: the conjugate of what was rotated
+    (got,) = torch.autograd.grad(torch.complex(r(q, k, p)[0], r(q, k, p)[0]).conj().imag.sum(), (q,))
+    (want,) = torch.autograd.grad(-r(q, k, p)[0].sum(), (q,))
+    assert torch.equal(got, want)
+    with forward_ad.dual_level():
+        out = r(forward_ad.make_dual(q.detach(), dq), forward_ad.make_dual(k.detach(), torch._efficientzerotensor(k.shape, device=DEV)), p)
+        assert torch.equal(forward_ad.unpack_dual(out[0]).tangent, r(dq.resolve_neg(), k, p)[0])
+        assert bool((forward_ad.unpack_dual(out[1]).tangent == 0).all())
+    # and in the cache
+    q, k = zq.imag.contiguous(), zk.imag.contiguous()
+    starts = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    caches = [da.PagedKVCache(1, 16, 2, 64, dtype=torch.float32) for _ in range(2)]
+    outs = []
+    for cache, a, b in ((caches[0], dense(q), dense(k)), (caches[1], -q, -k)):
+        outs.append((cache.append_(b, b, table, starts[1:], starts=starts, q=a, rotary=r), cache.attend(a[:1], table, starts[1:])))
+    assert torch.equal(caches[0].pages, caches[1].pages) and all(torch.equal(a, b) for a, b in zip(*outs))
